@@ -7,8 +7,9 @@
 All arithmetic runs in libfused_swiglu_sm100.so (sm_100a TMA + tcgen05 kernels);
 there is no Triton, PyTorch or CPU fallback.
 """
+from .router import FusedRouter, route
 from .swiglu import FusedSwiGLU
 from .swiglu_f16 import FastAccumFusedSwiGLU
 
-__all__ = ["FusedSwiGLU", "FastAccumFusedSwiGLU"]
+__all__ = ["FusedSwiGLU", "FastAccumFusedSwiGLU", "FusedRouter", "route"]
 __version__ = "0.1.0"

@@ -292,3 +292,49 @@ def wait_flags(flags_ptr: int, n: int, seq: int, like: torch.Tensor) -> None:
     with torch.cuda.device(like.device):
         rc = _lib.load().fsw_wait_flags(flags_ptr, int(n), int(seq) & 0xFFFFFFFF, _stream(like))
     _lib.check("fsw_wait_flags", rc)
+
+
+_ROUTE_DTYPE_CODE = {**_DTYPE_CODE, torch.float32: _lib.FSW_FP32}
+_SCORE_CODE = {"softmax": _lib.FSW_SCORE_SOFTMAX, "sigmoid": _lib.FSW_SCORE_SIGMOID}
+
+
+def _route_code(t: torch.Tensor) -> int:
+    try:
+        return _ROUTE_DTYPE_CODE[t.dtype]
+    except KeyError:
+        raise AssertionError(f"Expected bf16, fp16 or fp32 logits, got {t.dtype}") from None
+
+
+def route(logits: torch.Tensor, bias: Optional[torch.Tensor], top_k: int, score: str, renormalize: bool,
+          scale: float, num_groups: int, topk_groups: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(weights fp32, indices int32), each (T, top_k), for logits (T, E) whose rows may be
+    strided; bias (E,) or None."""
+    code = _route_code(logits)
+    _require_cuda(logits, *(() if bias is None else (bias,)))
+    T, E = logits.shape
+    if bias is not None:
+        bias = bias.detach().to(torch.float32).contiguous()
+    weights = torch.empty((T, max(top_k, 0)), device=logits.device, dtype=torch.float32)
+    indices = torch.empty((T, max(top_k, 0)), device=logits.device, dtype=torch.int32)
+    with torch.cuda.device(logits.device):
+        rc = _lib.load().fsw_route(
+            logits.data_ptr(), logits.stride(0) if T > 1 else E, bias.data_ptr() if bias is not None else None,
+            weights.data_ptr(), indices.data_ptr(), T, E, top_k, code, _SCORE_CODE[score], int(renormalize), scale,
+            num_groups, topk_groups, _stream(logits))
+    _lib.check("fsw_route", rc)
+    return weights, indices
+
+
+def route_backward(logits: torch.Tensor, indices: torch.Tensor, dweights: torch.Tensor, score: str,
+                   renormalize: bool, scale: float) -> torch.Tensor:
+    """d logits (T, E), in the logits' type, from the gradient of the fp32 weights."""
+    _require_cuda(logits, indices, dweights)
+    T, E = logits.shape
+    dlogits = torch.empty((T, E), device=logits.device, dtype=logits.dtype)
+    with torch.cuda.device(logits.device):
+        rc = _lib.load().fsw_route_backward(
+            logits.data_ptr(), logits.stride(0) if T > 1 else E, indices.data_ptr(), dweights.data_ptr(),
+            dlogits.data_ptr(), T, E, indices.shape[1], _route_code(logits), _SCORE_CODE[score], int(renormalize),
+            scale, _stream(logits))
+    _lib.check("fsw_route_backward", rc)
+    return dlogits

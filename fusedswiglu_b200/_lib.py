@@ -6,13 +6,14 @@ an exception is raised.  There is no PyTorch or CPU fallback.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_int, c_int64, c_uint32, c_uint64, c_void_p, POINTER
+from ctypes import c_char_p, c_float, c_int, c_int64, c_uint32, c_uint64, c_void_p, POINTER
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libfused_swiglu_sm100.so"
 
-FSW_BF16, FSW_FP16 = 0, 1
+FSW_BF16, FSW_FP16, FSW_FP32 = 0, 1, 2
 FSW_ACC_F32, FSW_ACC_F16 = 0, 1
+FSW_SCORE_SOFTMAX, FSW_SCORE_SIGMOID = 0, 1
 FSW_OK = 0
 
 # name -> (restype, argtypes); mirrors include/fused_swiglu.h one to one.
@@ -39,6 +40,8 @@ SIGNATURES = {
     "fsw_debug_split_work": (c_int, [c_int] * 7 + [POINTER(c_int64), POINTER(c_int)]),
     "fsw_debug_decode_tile": (c_int, [c_int] * 4 + [POINTER(c_int), POINTER(c_int)]),
     "fsw_debug_descriptors": (c_int, [c_int] * 6 + [POINTER(c_uint32), POINTER(c_uint64), POINTER(c_uint64)]),
+    "fsw_route": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64] + [c_int] * 5 + [c_float, c_int, c_int, c_void_p]),
+    "fsw_route_backward": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64] + [c_int] * 5 + [c_float, c_void_p]),
     "fsw_last_error": (c_char_p, []),
     "fsw_query_device": (c_int, [c_int, POINTER(c_int), POINTER(c_int), POINTER(c_int), POINTER(c_int64)]),
     "fsw_status": (c_int64, []),

@@ -18,26 +18,20 @@
 #include <mutex>
 
 #include "fsw_gemm.cuh"
+#include "fsw_host.h"
 
 namespace fsw {
 
 // ------------------------------------------------------------------ errors --
 static thread_local char t_err[512] = "";
 
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(t_err, sizeof(t_err), fmt, ap);
   va_end(ap);
   return code;
 }
-
-#define FSW_CUDA(call)                                                                   \
-  do {                                                                                   \
-    cudaError_t e_ = (call);                                                             \
-    if (e_ != cudaSuccess)                                                               \
-      return fail(FSW_ECUDA, "%s failed: %s", #call, cudaGetErrorString(e_));            \
-  } while (0)
 
 // ----------------------------------------------------------------- options --
 struct Options {
@@ -68,7 +62,12 @@ struct Options {
 };
 static Options g_opt;
 // Kernels this library has launched in this process (read through fsw_get_option("kernel_launches")).
-static std::atomic<long long> g_kernel_launches{0};
+std::atomic<long long> g_kernel_launches{0};
+int64_t opt_l2_a() { return g_opt.l2_a; }
+int64_t opt_l2_b() { return g_opt.l2_b; }
+int64_t opt_l2_out() { return g_opt.l2_out; }
+int64_t opt_wait_limit_ms() { return g_opt.wait_limit_ms; }
+int64_t opt_stall_producer() { return g_opt.stall_producer; }
 
 // Status word the kernels write when a bounded wait gives up.
 __device__ uint32_t g_status_word;
@@ -87,19 +86,6 @@ __device__ unsigned long long g_clk_probe[8];
 
 // ------------------------------------------------------------ device cache --
 constexpr int kMaxDevices = 64;
-struct DeviceInfo {
-  bool ready = false;
-  int sm_count = 0, cc_major = 0, cc_minor = 0;
-  int64_t smem_optin = 0;
-  int max_pairs = 0;  // co-resident 2-CTA clusters of the GEMM kernels
-  uint32_t* status = nullptr;
-  unsigned long long* clk_probe = nullptr;
-  unsigned int* pace = nullptr;
-  unsigned int* ew_ctrl = nullptr;
-  unsigned int ew_next = 0;     // next slot of g_ew_ctrl to hand out
-  unsigned int pace_next = 0;   // next slot of g_pace to hand out
-  unsigned int pace_last = 0;   // slot the last paced launch used
-};
 static DeviceInfo g_dev[kMaxDevices];
 static std::mutex g_mu;
 
@@ -124,7 +110,7 @@ static cudaError_t prepare_mode() {
   return prepare_kernel<MODE, CG, NSUB, __half, true>();
 }
 
-static int ensure_device(DeviceInfo** out) {
+int ensure_device(DeviceInfo** out) {
   int dev = 0;
   FSW_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= kMaxDevices) return fail(FSW_EINVAL, "device index %d out of range", dev);
@@ -230,13 +216,13 @@ static int ensure_device(DeviceInfo** out) {
 // a tensor of the same geometry.)
 struct MapKey {
   const void* ptr;
-  uint64_t inner, outer, row_elems;
+  uint64_t inner, outer, row_elems, depth;
   uint32_t box_inner, box_outer;
-  int32_t dtype, l2_promo;
+  int32_t dtype, l2_promo, elem_bytes;
   bool operator==(const MapKey& o) const {
     return ptr == o.ptr && inner == o.inner && outer == o.outer && row_elems == o.row_elems &&
-           box_inner == o.box_inner && box_outer == o.box_outer && dtype == o.dtype &&
-           l2_promo == o.l2_promo;
+           depth == o.depth && box_inner == o.box_inner && box_outer == o.box_outer &&
+           dtype == o.dtype && l2_promo == o.l2_promo && elem_bytes == o.elem_bytes;
   }
 };
 constexpr int kMapCacheSlots = 256;
@@ -252,7 +238,8 @@ static uint64_t g_map_hits = 0, g_map_misses = 0;
 static uint32_t map_slot(const MapKey& k) {
   uint64_t h = reinterpret_cast<uintptr_t>(k.ptr) * 0x9E3779B97F4A7C15ull;
   h ^= (k.inner * 0xC2B2AE3D27D4EB4Full) ^ (k.outer * 0x165667B19E3779F9ull) ^
-       (k.row_elems * 0x27D4EB2F165667C5ull) ^
+       (k.row_elems * 0x27D4EB2F165667C5ull) ^ (k.depth * 0x9E3779B185EBCA87ull) ^
+       ((uint64_t)k.elem_bytes << 20) ^
        ((uint64_t)k.box_outer << 40) ^ ((uint64_t)k.box_inner << 32) ^ ((uint64_t)k.dtype << 8) ^
        (uint64_t)k.l2_promo;
   h ^= h >> 29;
@@ -261,14 +248,11 @@ static uint32_t map_slot(const MapKey& k) {
   return (uint32_t)(h % kMapCacheSlots);
 }
 
-// Row-major (outer, inner) array of 16-bit elements; box = box_outer rows of 64
-// elements (128 bytes, 128-byte swizzle) or of 32 elements (64 bytes, 64-byte swizzle).
-// `row_elems` is the distance between rows in elements when the map covers a column
-// range of a wider array (0 = dense, rows are `inner` elements apart).
-static int make_map(CUtensorMap* m, const void* ptr, int dtype, uint64_t inner, uint64_t outer,
-                    uint32_t box_outer, const char* what, uint32_t box_inner = 64,
-                    uint64_t row_elems = 0) {
-  const MapKey key = {ptr, inner, outer, row_elems, box_inner, box_outer, dtype, (int32_t)g_opt.l2_promo};
+int make_map(CUtensorMap* m, const void* ptr, int dtype, uint64_t inner, uint64_t outer,
+             uint32_t box_outer, const char* what, uint32_t box_inner, uint64_t row_elems,
+             uint64_t depth, int elem_bytes) {
+  const MapKey key = {ptr, inner, outer, row_elems, depth, box_inner, box_outer, dtype,
+                      (int32_t)g_opt.l2_promo, elem_bytes};
   const uint32_t slot = map_slot(key);
   {
     std::lock_guard<std::mutex> lock(g_map_mu);
@@ -279,14 +263,18 @@ static int make_map(CUtensorMap* m, const void* ptr, int dtype, uint64_t inner, 
       return FSW_OK;
     }
   }
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {(row_elems ? row_elems : inner) * 2};
-  cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
+  const uint64_t row_bytes = (row_elems ? row_elems : inner) * (uint64_t)elem_bytes;
+  cuuint64_t dims[3] = {inner, outer, depth};
+  cuuint64_t strides[2] = {row_bytes, row_bytes * outer};
+  cuuint32_t box[3] = {box_inner, box_outer, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType type = elem_bytes == 1      ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : dtype == FSW_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUresult r = g_encode(
-      m, dtype == FSW_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-      const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-      box_inner == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+      m, type, depth ? 3 : 2, const_cast<void*>(ptr), dims, strides, box, estr,
+      CU_TENSOR_MAP_INTERLEAVE_NONE,
+      box_inner * (uint32_t)elem_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
       key.l2_promo == 0   ? CU_TENSOR_MAP_L2_PROMOTION_NONE
       : key.l2_promo == 1 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
                           : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -307,7 +295,7 @@ static int make_map(CUtensorMap* m, const void* ptr, int dtype, uint64_t inner, 
 
 // UMMA instruction descriptor, kind::f16: D format [4,6), A format [7,10),
 // B format [10,13), A major bit 15, B major bit 16, N>>3 at [17,23), M>>4 at [24,29).
-static uint32_t make_idesc(int dtype, bool acc16, int a_major, int b_major, int m, int n) {
+uint32_t make_idesc(int dtype, bool acc16, int a_major, int b_major, int m, int n) {
   uint32_t d = 0;
   d |= (acc16 ? 0u : 1u) << 4;
   d |= (dtype == FSW_BF16 ? 1u : 0u) << 7;
@@ -322,7 +310,7 @@ static uint32_t make_idesc(int dtype, bool acc16, int a_major, int b_major, int 
 // UMMA shared-memory descriptor without the start address: leading byte offset
 // at [16,30), stride byte offset at [32,46) (both >>4), version 1 at bit 46,
 // layout type SWIZZLE_128B (2) at [61,64).
-static uint64_t make_sdesc(uint32_t lbo_bytes, uint32_t sbo_bytes) {
+uint64_t make_sdesc(uint32_t lbo_bytes, uint32_t sbo_bytes) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFFu) << 16;
   d |= static_cast<uint64_t>((sbo_bytes >> 4) & 0x3FFFu) << 32;
@@ -331,7 +319,7 @@ static uint64_t make_sdesc(uint32_t lbo_bytes, uint32_t sbo_bytes) {
   return d;
 }
 
-static void fill_operand_desc(int major, uint64_t* desc, uint32_t* kadv) {
+void fill_operand_desc(int major, uint64_t* desc, uint32_t* kadv) {
   if (major == MAJOR_K) {
     // rows of 64 elements = one 128-byte swizzle row; 8-row groups 1024 B apart;
     // a K=16 step moves 32 bytes inside the swizzle row.
@@ -372,8 +360,6 @@ static cudaError_t launch_cg(const GemmParams& p, int grid, int dtype, bool acc1
   if (acc16) return launch_one<MODE, CG, NSUB, __half, true>(p, grid, st);
   return launch_one<MODE, CG, NSUB, __half, false>(p, grid, st);
 }
-
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 static int check_common(int64_t T, int64_t dm, int64_t di, int dtype, int accum) {
   if (dtype != FSW_BF16 && dtype != FSW_FP16) return fail(FSW_EINVAL, "unknown dtype %d", dtype);

@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-enum { FSW_BF16 = 0, FSW_FP16 = 1 };
+enum { FSW_BF16 = 0, FSW_FP16 = 1, FSW_FP32 = 2 /* routing only */ };
 enum { FSW_ACC_F32 = 0, FSW_ACC_F16 = 1 };
 enum {
   FSW_OK = 0,
@@ -254,6 +254,33 @@ int fsw_backward_static_scratch(const void* dout, const void* x, const void* w_g
                                 const void* w_up, const void* g, const void* u, void* dx,
                                 void* dw_gate, void* dw_up, int64_t T, int64_t dm, int64_t di,
                                 int dtype, int accum, void* stream);
+
+/*
+ * Routing of tokens to experts (mixture-of-experts layers; no counterpart in the
+ * reference).  logits: (T, E) of `dtype` (FSW_FP32 too), rows `ld` elements apart.
+ *   s = softmax(logits) or sigmoid(logits);  c = s + bias (bias: E floats or NULL; it
+ *   steers the selection only and gets no gradient);
+ *   num_groups > 1 (it divides E, at most 32): a group's score is the sum of its two
+ *   largest c, and only experts of the topk_groups best groups stay eligible;
+ *   indices (T, k) int32: the k largest c in descending order, ties to the lowest
+ *   index - as exact arithmetic would order them, whatever the rounding of s;
+ *   weights (T, k) fp32: scale * s[indices], divided by their sum if `renormalize`.
+ * A logit of -inf is a mask: such an expert is picked only when nothing else is eligible,
+ * and its weight is 0; in a row without anything else all weights are 0.  NaN ranks with
+ * the masked experts; NaN or +inf in a softmax row makes the row's weights NaN.  Indices
+ * are always distinct and in range.  E <= FSW_MAX_EXPERTS, k <= FSW_MAX_TOP_K.
+ * fsw_route_backward: dlogits (T, E), dense, of `dtype`, from dweights (T, k) fp32 and the
+ * forward's indices.  Pointers need only their element's alignment.
+ */
+enum { FSW_SCORE_SOFTMAX = 0, FSW_SCORE_SIGMOID = 1 };
+#define FSW_MAX_EXPERTS 1024
+#define FSW_MAX_TOP_K 32
+int fsw_route(const void* logits, int64_t ld, const void* bias, void* weights, void* indices,
+              int64_t T, int E, int k, int dtype, int score, int renormalize, float scale,
+              int num_groups, int topk_groups, void* stream);
+int fsw_route_backward(const void* logits, int64_t ld, const void* indices, const void* dweights,
+                       void* dlogits, int64_t T, int E, int k, int dtype, int score,
+                       int renormalize, float scale, void* stream);
 
 /* Message for the last non-zero return on the calling thread ("" if none). */
 const char* fsw_last_error(void);
