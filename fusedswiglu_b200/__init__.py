@@ -7,9 +7,11 @@
 All arithmetic runs in libfused_swiglu_sm100.so (sm_100a TMA + tcgen05 kernels);
 there is no Triton, PyTorch or CPU fallback.
 """
+from .experts import FusedSwiGLUExperts, SwiGLUMoE
 from .router import FusedRouter, route
 from .swiglu import FusedSwiGLU
 from .swiglu_f16 import FastAccumFusedSwiGLU
 
-__all__ = ["FusedSwiGLU", "FastAccumFusedSwiGLU", "FusedRouter", "route"]
+__all__ = ["FusedSwiGLU", "FastAccumFusedSwiGLU", "FusedRouter", "route",
+           "FusedSwiGLUExperts", "SwiGLUMoE"]
 __version__ = "0.1.0"

@@ -5,6 +5,8 @@ every arithmetic result comes from libfused_swiglu_sm100.so.
 """
 from __future__ import annotations
 
+import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -338,3 +340,75 @@ def route_backward(logits: torch.Tensor, indices: torch.Tensor, dweights: torch.
             scale, _stream(logits))
     _lib.check("fsw_route_backward", rc)
     return dlogits
+
+
+def expert_indices(indices: torch.Tensor, num_experts: int) -> torch.Tensor:
+    """(T, k) int32, contiguous; wider indices are clamped first so that none wraps into range."""
+    idx = indices.reshape(-1, indices.shape[-1])
+    if idx.dtype != torch.int32:
+        idx = idx.clamp(-1, num_experts).to(torch.int32)
+    return idx.contiguous()
+
+
+@functools.lru_cache(maxsize=1024)
+def _expert_sizes(T: int, k: int, E: int, d: int, f: int, d_out: int) -> Tuple[int, int, int, int]:
+    out = (ctypes.c_int64 * 4)()
+    at = [ctypes.cast(ctypes.byref(out, 8 * i), ctypes.POINTER(ctypes.c_int64)) for i in range(4)]
+    _lib.check("fsw_experts_sizes", _lib.load().fsw_experts_sizes(T, k, E, d, f, d_out, *at))
+    return tuple(out)
+
+
+def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
+    return torch.empty(max(nbytes, 16), device=like.device, dtype=torch.uint8)
+
+
+def _weights_code(weights: torch.Tensor, like: torch.Tensor) -> int:
+    return _lib.FSW_FP32 if weights.dtype == torch.float32 else _code(like)
+
+
+def experts_forward(x: torch.Tensor, weights: torch.Tensor, indices: torch.Tensor, w_gate: torch.Tensor,
+                    w_up: torch.Tensor, w_down: torch.Tensor, *, save: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """y (T, d_out) and, with ``save``, the buffer the backward reads."""
+    _require_cuda(x, weights, indices, w_gate, w_up, w_down)
+    (T, d), k = x.shape, weights.shape[1]
+    E, _, f = w_gate.shape
+    d_out = w_down.shape[2]
+    code = _code(x)
+    saved_bytes, forward_bytes, inference_bytes, _ = _expert_sizes(T, k, E, d, f, d_out)
+    y = torch.empty((T, d_out), device=x.device, dtype=x.dtype)
+    saved = _scratch(saved_bytes, x) if save else None
+    nbytes = forward_bytes if save else inference_bytes
+    scratch = _scratch(nbytes, x)
+    with torch.cuda.device(x.device):
+        rc = _lib.load().fsw_experts_forward(
+            x.data_ptr(), weights.data_ptr(), indices.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+            w_down.data_ptr(), y.data_ptr(), saved.data_ptr() if save else None, saved_bytes if save else 0,
+            scratch.data_ptr(), nbytes, T, k, E, d, f, d_out, code, _weights_code(weights, x), _stream(x))
+    _lib.check("fsw_experts_forward", rc)
+    return y, saved
+
+
+def experts_backward(dy: torch.Tensor, weights: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+                     w_down: torch.Tensor, saved: torch.Tensor, *, need_x: bool, need_weights: bool,
+                     need_gate_up: bool, need_down: bool):
+    """(dx, dweights, dw_gate, dw_up, dw_down); None where not needed."""
+    _require_cuda(dy, weights, w_gate, w_up, w_down, saved)
+    if dy.dtype != w_gate.dtype:
+        dy = dy.to(w_gate.dtype)
+    T, k = weights.shape
+    E, d, f = w_gate.shape
+    d_out = w_down.shape[2]
+    saved_bytes, _, _, backward_bytes = _expert_sizes(T, k, E, d, f, d_out)
+    scratch = _scratch(backward_bytes, dy)
+    dx = torch.empty((T, d), device=dy.device, dtype=dy.dtype) if need_x else None
+    dr = torch.empty_like(weights) if need_weights else None
+    dwg, dwu = (torch.empty_like(w_gate), torch.empty_like(w_up)) if need_gate_up else (None, None)
+    dwd = torch.empty_like(w_down) if need_down else None
+    ptr = lambda t: t.data_ptr() if t is not None else None
+    with torch.cuda.device(dy.device):
+        rc = _lib.load().fsw_experts_backward(
+            dy.data_ptr(), weights.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
+            saved.data_ptr(), saved_bytes, scratch.data_ptr(), backward_bytes, ptr(dx), ptr(dr), ptr(dwg), ptr(dwu),
+            ptr(dwd), T, k, E, d, f, d_out, _code(dy), _weights_code(weights, dy), _stream(dy))
+    _lib.check("fsw_experts_backward", rc)
+    return dx, dr, dwg, dwu, dwd

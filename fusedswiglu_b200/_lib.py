@@ -42,6 +42,9 @@ SIGNATURES = {
     "fsw_debug_descriptors": (c_int, [c_int] * 6 + [POINTER(c_uint32), POINTER(c_uint64), POINTER(c_uint64)]),
     "fsw_route": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64] + [c_int] * 5 + [c_float, c_int, c_int, c_void_p]),
     "fsw_route_backward": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64] + [c_int] * 5 + [c_float, c_void_p]),
+    "fsw_experts_sizes": (c_int, [c_int64, c_int, c_int] + [c_int64] * 3 + [POINTER(c_int64)] * 4),
+    "fsw_experts_forward": (c_int, [c_void_p] * 8 + [c_int64, c_void_p, c_int64, c_int64, c_int, c_int] + [c_int64] * 3 + [c_int, c_int, c_void_p]),
+    "fsw_experts_backward": (c_int, [c_void_p] * 6 + [c_int64, c_void_p, c_int64] + [c_void_p] * 5 + [c_int64, c_int, c_int] + [c_int64] * 3 + [c_int, c_int, c_void_p]),
     "fsw_last_error": (c_char_p, []),
     "fsw_query_device": (c_int, [c_int, POINTER(c_int), POINTER(c_int), POINTER(c_int), POINTER(c_int64)]),
     "fsw_status": (c_int64, []),

@@ -1,0 +1,72 @@
+// Layout of the rows of a mixture of experts, shared by the 16-bit and the 8-bit products.
+//
+// The T*k (token, expert) pairs are sorted by expert, stably, and every expert's rows start
+// at a multiple of `tile_rows`, so that a tile of the GEMM kernels has one expert and none
+// is cut by a boundary.  The host knows only the bound `rows` on their number; the kernels
+// read the rest from the plan, an int32 array in device memory:
+//   meta[8]            [0] row tiles in use, [1] rows in use (padding included)
+//   counts[E]          rows of each expert (without padding)
+//   offsets[E + 1]     first row of each expert
+//   tile_expert[tiles] expert of each row tile
+//   pair_row[T*k]      row of each pair, -1 for an index outside [0, E)
+//   row_pair[rows]     pair of each row, -1 for padding
+//   block_hist         scratch of the sort
+#pragma once
+
+#include "fsw_host.h"
+
+namespace fsw {
+
+constexpr int kPlanChunk = 4096;   // pairs sorted by one block
+constexpr int kPlanWarps = 8;      // warps of a sorting block
+
+struct ExpertPlan {
+  int T, k, E, tile_rows;
+  int pairs, tiles, rows, blocks;
+  // offsets into the plan, in ints
+  int64_t counts, offsets, tile_expert, pair_row, row_pair, block_hist, ints;
+};
+
+// Fills `p`; false if the rows do not fit 31 bits.
+inline bool make_plan(ExpertPlan* p, int64_t T, int k, int E, int tile_rows) {
+  const int64_t pairs = T * k;
+  const int64_t used = pairs < E ? pairs : E;
+  const int64_t tiles = (pairs + used * (tile_rows - 1)) / tile_rows;
+  if (pairs >= (1ll << 31) || tiles * tile_rows >= (1ll << 31) - 1024) return false;
+  p->T = (int)T;
+  p->k = k;
+  p->E = E;
+  p->tile_rows = tile_rows;
+  p->pairs = (int)pairs;
+  p->tiles = (int)tiles;
+  p->rows = (int)(tiles * tile_rows);
+  p->blocks = (int)((pairs + kPlanChunk - 1) / kPlanChunk);
+  p->counts = 8;
+  p->offsets = p->counts + E;
+  p->tile_expert = p->offsets + E + 1;
+  p->pair_row = p->tile_expert + tiles;
+  p->row_pair = p->pair_row + pairs;
+  p->block_hist = p->row_pair + p->rows;
+  p->ints = p->block_hist + (int64_t)p->blocks * E;
+  return true;
+}
+
+// Height of a row tile: 256 rows (a CTA pair) if an expert has enough rows on average to
+// fill such tiles, else 128.
+inline int choose_tile_rows(int64_t pairs, int E) { return pairs >= 256ll * E ? 256 : 128; }
+
+// Sorts the pairs (launches on `st`).
+int build_plan(const ExpertPlan& p, const int* indices, int* plan, cudaStream_t st);
+
+// dst[row] = src[token of row] for 16-byte multiples of `row_bytes`; optionally zeros the padding.
+int gather_rows(const ExpertPlan& p, const int* plan, const void* src, void* dst, int64_t row_bytes,
+                bool zero_padding, cudaStream_t st);
+
+// y[t] = sum over j of weight[t, j] * src[row of (t, j)], in fp32, rounded once.
+// weights: nullptr for 1, else of type wtype (FSW_FP32 or dtype).
+int combine_rows(const ExpertPlan& p, const int* plan, const void* src, const void* weights, int wtype, void* y,
+                 int64_t cols, int dtype, cudaStream_t st);
+
+int check_experts(int64_t T, int k, int E, int64_t d, int64_t f, int64_t d_out, int dtype, int wtype);
+
+}  // namespace fsw

@@ -18,6 +18,13 @@
 //   MODE_NT  : A (M,K) @ B (N,K)^T    (A K-major,  B K-major)
 //   MODE_TN  : A (K,M)^T @ B (K,N)    (A MN-major, B MN-major)
 //
+// The MODE_G* modes are the products of a mixture of experts: FWD, NN, NT, DX, DW and TN
+// with one weight (or weight gradient) per expert and rows sorted by expert.  Every
+// expert's rows start at a multiple of the tile height, so a tile has one expert; which, and
+// how many tiles there are, is read from device memory (GemmParams::grp_*).  The weights
+// are rank-3 tensor maps.  In the gradients of the weights (GDW, GTN) an expert's rows are
+// the K range of its tiles; rows between its last and the next tile boundary hold zeros.
+//
 // One CTA owns 128 rows x 512 fp32 columns of tensor memory, used as two
 // 256-column accumulator regions.
 //   NSUB == 1: a tile is 128 x 256 per CTA; the two regions alternate between
@@ -51,13 +58,23 @@
 
 namespace fsw {
 
-enum : int { MODE_FWD = 0, MODE_DX = 1, MODE_DW = 2, MODE_NN = 3, MODE_NT = 4, MODE_TN = 5, MODE_DXG = 6, MODE_FWDST = 7, MODE_DXE = 8 };
+enum : int { MODE_FWD = 0, MODE_DX = 1, MODE_DW = 2, MODE_NN = 3, MODE_NT = 4, MODE_TN = 5, MODE_DXG = 6, MODE_FWDST = 7, MODE_DXE = 8,
+             MODE_GFWD = 9, MODE_GNN = 10, MODE_GNT = 11, MODE_GDX = 12, MODE_GDW = 13, MODE_GTN = 14 };
 // MODE_FWDST is MODE_FWD that saves s = silu(g) and t = u * silu'(g) where g and u would go.
-__host__ __device__ constexpr bool is_fwd(int mode) { return mode == MODE_FWD || mode == MODE_FWDST; }
+__host__ __device__ constexpr bool is_fwd(int mode) { return mode == MODE_FWD || mode == MODE_FWDST || mode == MODE_GFWD; }
 // MODE_DXE is MODE_DX whose otherwise idle epilogue warps also do the gate-gradient
 // elementwise step (dg, du from dout, g, u), once per element, ahead of the tiles that
 // read dg and du through TMA; see GemmParams::ew_*.
-__host__ __device__ constexpr bool is_dx(int mode) { return mode == MODE_DX || mode == MODE_DXE; }
+__host__ __device__ constexpr bool is_dx(int mode) { return mode == MODE_DX || mode == MODE_DXE || mode == MODE_GDX; }
+__host__ __device__ constexpr bool is_dw(int mode) { return mode == MODE_DW || mode == MODE_GDW; }
+__host__ __device__ constexpr bool is_grouped(int mode) { return mode >= MODE_GFWD; }
+// the experts' rows are the K dimension (weight gradients), not the M dimension
+__host__ __device__ constexpr bool is_grouped_k(int mode) { return mode == MODE_GDW || mode == MODE_GTN; }
+__host__ __device__ constexpr bool a_is_mn(int mode) { return is_dw(mode) || mode == MODE_TN || mode == MODE_GTN; }
+__host__ __device__ constexpr bool b_is_k(int mode) {
+  return is_dx(mode) || mode == MODE_NT || mode == MODE_GNT || mode == MODE_DXG;
+}
+__host__ __device__ constexpr bool is_dual(int mode) { return is_fwd(mode) || is_dw(mode); }
 enum : int { MAJOR_K = 0, MAJOR_MN = 1 };
 
 // Codes written to the status word when a bounded wait gives up.
@@ -147,6 +164,14 @@ struct GemmParams {
   // queue behind them.  Spread over most of a tile's K loop the same bytes never
   // exceed the link's rate.
   unsigned int scatter_gap_ns;
+  // MODE_G*: num_m_tiles is read from grp_meta[0] (row-grouped modes); expert of each row
+  // tile, first row and number of rows of each expert.
+  const int *grp_meta, *grp_tile_expert, *grp_offsets, *grp_counts;
+  int grp_experts;
+  // Rows of an A box in the row-grouped modes (0 = 128).  With a handful of rows in all,
+  // no tile has more than that many; the rest of the stage is left stale, and so are the
+  // accumulator rows behind it, which only rows behind an expert's last receive.
+  int grp_a_rows;
   // Tile rows are visited starting at row tile m_rotate (mod num_m_tiles): with the
   // scatter every rank starts at another owner's rows, so that at any moment the
   // ranks store to different GPUs instead of all to the same one.
@@ -159,6 +184,7 @@ constexpr int kMaxScatterRanks = 8;
 // sum that goes to workspace slot `slot`.
 struct WorkItem {
   int m_tile, n_tile, it0, it1, slot;
+  int expert;  // MODE_G* only
 };
 constexpr int kSplitSlotFloats = 2 * 128 * 512;  // one slot: both CTAs' 128 x 512 accumulators
 
@@ -195,12 +221,12 @@ constexpr int kSmemBudget = 232448;  // 227 KB opt-in limit per CTA
 template <int MODE, int CG, int NSUB>
 struct TileCfg {
   static_assert(NSUB == 1 || (NSUB == 2 && CG == 2), "512-column tiles need a CTA pair");
-  static constexpr int A_MAJOR = (MODE == MODE_DW || MODE == MODE_TN) ? MAJOR_MN : MAJOR_K;
-  static constexpr int B_MAJOR = (is_dx(MODE) || MODE == MODE_NT || MODE == MODE_DXG) ? MAJOR_K : MAJOR_MN;
+  static constexpr int A_MAJOR = a_is_mn(MODE) ? MAJOR_MN : MAJOR_K;
+  static constexpr int B_MAJOR = b_is_k(MODE) ? MAJOR_K : MAJOR_MN;
   // the A operand is written by the epilogue warps instead of TMA
   static constexpr bool A_BY_WARPS = (MODE == MODE_DXG);
   // dual: the accumulator columns of a region are [128 from b0 | 128 from b1]
-  static constexpr bool DUAL_B = (is_fwd(MODE) || MODE == MODE_DW);
+  static constexpr bool DUAL_B = is_dual(MODE);
   static constexpr int BM = 128;          // accumulator rows per CTA
   static constexpr int BN = 256;          // columns of one accumulator region (MMA N)
   static constexpr int BK = 64;           // one 128-byte swizzle row of 16-bit elements
@@ -395,6 +421,28 @@ __host__ __device__ __forceinline__ bool next_work(const GemmParams& p, int iter
   return true;
 }
 
+// The same for the MODE_G* modes; num_m_tiles is grp_meta[0] in the row-grouped ones.
+template <bool BY_K>
+__device__ __forceinline__ bool next_group_work(const GemmParams& p, int num_m_tiles, int iters_per_tile,
+                                                int cluster_id, int num_clusters, int idx, WorkItem& w) {
+  const long long t = cluster_id + static_cast<long long>(idx) * num_clusters;
+  const long long per = static_cast<long long>(num_m_tiles) * p.num_n_tiles;
+  w.slot = -1;
+  if (BY_K) {
+    if (t >= per * p.grp_experts) return false;
+    w.expert = static_cast<int>(t / per);
+    decode_tile_order(static_cast<int>(t - w.expert * per), num_m_tiles, p.num_n_tiles, p.group_m, w.m_tile, w.n_tile);
+    w.it0 = p.grp_offsets[w.expert] / 64;
+    w.it1 = w.it0 + (p.grp_counts[w.expert] + 63) / 64;
+  } else {
+    if (t >= per) return false;
+    decode_tile_order(static_cast<int>(t), num_m_tiles, p.num_n_tiles, p.group_m, w.m_tile, w.n_tile);
+    w.expert = p.grp_tile_expert[w.m_tile];
+    w.it0 = 0;
+    w.it1 = iters_per_tile;
+  }
+  return true;
+}
 
 // ---------------------------------------------------------------- epilogue --
 // tcgen05.ld hands every thread 32 consecutive columns of ONE accumulator row, so
@@ -622,7 +670,7 @@ __device__ __forceinline__ void drain_swiglu(const GemmParams& p, const EpiCtx& 
 // (the multi-GPU scatter writes them to peer memory over NVLink).
 template <class C, int MODE, typename T, bool ACC16, int NJB, class Release>
 __device__ __forceinline__ void drain_plain(const GemmParams& p, const EpiCtx& e, uint32_t taddr,
-                                            int n0, int jb_begin, Release release) {
+                                            int n0, int jb_begin, Release release, size_t out_offset = 0) {
   uint32_t pk[NJB * 32];
   auto read_box = [&](int j) {
 #pragma unroll
@@ -649,8 +697,9 @@ __device__ __forceinline__ void drain_plain(const GemmParams& p, const EpiCtx& e
 #pragma unroll
   for (int j = 0; j < NJB; ++j) {
     const int jb = jb_begin + j;
-    const int col = (MODE == MODE_DW) ? (n0 + (jb & 1) * 64) : (n0 + jb * 64);
-    void* out = (MODE == MODE_DW && jb >= 2) ? p.c1_ptr : p.c0_ptr;
+    const int col = is_dw(MODE) ? (n0 + (jb & 1) * 64) : (n0 + jb * 64);
+    void* out = (is_dw(MODE) && jb >= 2) ? p.c1_ptr : p.c0_ptr;
+    if (is_grouped_k(MODE)) out = static_cast<char*>(out) + out_offset;
     if (is_dx(MODE) && p.scatter_world > 1) out = scatter_out;
     if (FSW_PLAIN_ONE_PHASE) {  // measurement build: read, release after the last read, store box by box
       read_box(j);
@@ -660,6 +709,23 @@ __device__ __forceinline__ void drain_plain(const GemmParams& p, const EpiCtx& e
     __syncwarp();
     flush_rows128(e.buf, e.lane, out, e.row0, col, p.M, p.N, p.ldc, gap_ns);
     __syncwarp();
+  }
+}
+
+// The gradient of an expert without rows: its tile's boxes are zero.
+template <int MODE, int NJB>
+__device__ __forceinline__ void store_zeros(const GemmParams& p, const EpiCtx& e, int n0, int jb_begin,
+                                            size_t out_offset) {
+#pragma unroll
+  for (int j = 0; j < NJB; ++j) {
+    const int jb = jb_begin + j;
+    const int col0 = (is_dw(MODE) ? (n0 + (jb & 1) * 64) : (n0 + jb * 64)) + (e.lane & 7) * 8;
+    char* out = static_cast<char*>((is_dw(MODE) && jb >= 2) ? p.c1_ptr : p.c0_ptr) + out_offset;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = e.row0 + 4 * i + (e.lane >> 3);
+      if (row < p.M && col0 < p.N) ptx::st_global_v4(out + (static_cast<size_t>(row) * p.ldc + col0) * 2, 0u, 0u, 0u, 0u);
+    }
   }
 }
 
@@ -911,6 +977,14 @@ __global__ void __launch_bounds__(64 + 32 * FSW_EPI_WARPS, 1)
   const int cluster_id = blockIdx.x / CG;
   const int num_tiles = p.num_m_tiles * p.num_n_tiles;
   const int num_kb = p.num_k_blocks;
+  // The idx-th work item of this pair; the roles of both CTAs walk the same sequence.
+  const int grp_m_tiles = (is_grouped(MODE) && !is_grouped_k(MODE)) ? p.grp_meta[0] : p.num_m_tiles;
+  auto get_work = [&](int idx, WorkItem& w) {
+    if constexpr (is_grouped(MODE))
+      return next_group_work<is_grouped_k(MODE)>(p, grp_m_tiles, C::NSEG * num_kb, cluster_id, num_clusters, idx, w);
+    else
+      return next_work(p, C::NSEG * num_kb, cluster_id, num_clusters, idx, w);
+  };
 
   if (warp == 0) {
     // ======================= TMA producer (one thread) =======================
@@ -926,7 +1000,10 @@ __global__ void __launch_bounds__(64 + 32 * FSW_EPI_WARPS, 1)
       const unsigned int meets_per_tile =
           pacer.on ? static_cast<unsigned int>((kb_per_tile + pacer.kb - 1) / pacer.kb) : 0u;
       WorkItem w;
-      for (int idx = 0; ok && next_work(p, kb_per_tile, cluster_id, num_clusters, idx, w); ++idx) {
+      const uint32_t a_bytes = (is_grouped(MODE) && !is_grouped_k(MODE) && p.grp_a_rows)
+                                   ? static_cast<uint32_t>(p.grp_a_rows) * 128u
+                                   : static_cast<uint32_t>(C::A_BYTES);
+      for (int idx = 0; ok && get_work(idx, w); ++idx) {
         const int m0 = w.m_tile * C::TILE_M + cta_rank * C::BM;
         const int n0 = w.n_tile * C::TILE_N;
         if (MODE == MODE_DXE && w.m_tile != ew_ready_tile) {
@@ -984,7 +1061,7 @@ __global__ void __launch_bounds__(64 + 32 * FSW_EPI_WARPS, 1)
               ptx::mbar_arrive_expect_tx(full_bar(s),
                                          CG * (FSW_DBG_SKIP_B_LOADS ? C::A_BYTES
                                                : C::A_BY_WARPS      ? C::B_BYTES
-                                                                    : C::STAGE_BYTES));
+                                                                    : a_bytes + C::B_BYTES));
             auto load_pol = [&](uint32_t dst, const CUtensorMap* tm, int x, int y, uint64_t pol) {
               if (CG == 2)
                 ptx::tma_load_2d_pair(dst, tm, fb, x, y, pol);
@@ -995,7 +1072,14 @@ __global__ void __launch_bounds__(64 + 32 * FSW_EPI_WARPS, 1)
               load_pol(dst, tm, x, y, pol_a);
             };
             auto load = [&](uint32_t dst, const CUtensorMap* tm, int x, int y) {
-              load_pol(dst, tm, x, y, pol_b);
+              if constexpr (is_grouped(MODE) && !is_grouped_k(MODE)) {
+                if (CG == 2)
+                  ptx::tma_load_3d_pair(dst, tm, fb, x, y, w.expert, pol_b);
+                else
+                  ptx::tma_load_3d(dst, tm, fb, x, y, w.expert, pol_b);
+              } else {
+                load_pol(dst, tm, x, y, pol_b);
+              }
             };
             // ---- A tile: 128 rows x 64 k
             if (C::A_BY_WARPS) {
@@ -1055,7 +1139,8 @@ __global__ void __launch_bounds__(64 + 32 * FSW_EPI_WARPS, 1)
           ptx::mma_commit(bar);
       };
       WorkItem w;
-      for (int idx = 0; ok && next_work(p, C::NSEG * num_kb, cluster_id, num_clusters, idx, w); ++idx) {
+      for (int idx = 0; ok && get_work(idx, w); ++idx) {
+        if (is_grouped_k(MODE) && w.it0 == w.it1) continue;  // an expert without rows: no accumulation
         if (NSUB == 1) {
           ok = bounded_wait_thread(tempty_bar(a), aph ^ 1u, ctl, WAIT_MMA_TMEM_EMPTY);
           if (!ok) break;
@@ -1132,9 +1217,22 @@ __global__ void __launch_bounds__(64 + 32 * FSW_EPI_WARPS, 1)
                                       : 0u;
     long long prof_wait = 0, prof_drain = 0, prof_t0 = 0, prof_tiles = 0;
     WorkItem w;
-    for (int idx = 0; ok && next_work(p, C::NSEG * num_kb, cluster_id, num_clusters, idx, w); ++idx) {
+    for (int idx = 0; ok && get_work(idx, w); ++idx) {
       e.row0 = w.m_tile * C::TILE_M + cta_rank * C::BM + q * 32;
       const int n0 = w.n_tile * C::TILE_N;
+      // no row of this lane quadrant was loaded: nothing of it is stored
+      if (is_grouped(MODE) && !is_grouped_k(MODE) && p.grp_a_rows && q * 32 >= p.grp_a_rows) e.row0 = p.M;
+      const size_t out_offset =
+          is_grouped_k(MODE) ? static_cast<size_t>(w.expert) * static_cast<size_t>(p.M) * p.ldc * 2 : 0;
+      if (is_grouped_k(MODE) && w.it0 == w.it1) {
+        if (NSUB == 1) {
+          store_zeros<MODE, 4 / kSplit>(p, e, n0, kSplit == 2 ? 2 * chalf : 0, out_offset);
+        } else {
+          for (int r = (kSplit == 2 ? chalf : 0); r < (kSplit == 2 ? chalf + 1 : 2); ++r)
+            store_zeros<MODE, 4>(p, e, n0 + r * C::REGION_N, 0, out_offset);
+        }
+        continue;
+      }
       if (C::A_BY_WARPS) {
         // Produce this item's A tiles: dg = dout * t for the first num_kb iterations,
         // du = dout * s for the rest.  Loads run kPrefetch iterations ahead of their use.
@@ -1251,9 +1349,9 @@ __global__ void __launch_bounds__(64 + 32 * FSW_EPI_WARPS, 1)
             drain_swiglu<C, T, ACC16, 2, MODE == MODE_FWDST>(p, e, taddr, rn0, 0, release);
         } else {
           if (split)
-            drain_plain<C, MODE, T, ACC16, 2>(p, e, taddr, rn0, 2 * chalf, release);
+            drain_plain<C, MODE, T, ACC16, 2>(p, e, taddr, rn0, 2 * chalf, release, out_offset);
           else
-            drain_plain<C, MODE, T, ACC16, 4>(p, e, taddr, rn0, 0, release);
+            drain_plain<C, MODE, T, ACC16, 4>(p, e, taddr, rn0, 0, release, out_offset);
         }
       }
       if (FSW_PROFILE) prof_drain += clock64() - prof_t0;
@@ -1533,7 +1631,7 @@ __global__ void __launch_bounds__(256)
 
 // Time-limited wait until every word of flags[0..n) has reached `seq`; used to learn
 // that the peers' copies of their reduced rows into this rank's buffer have landed.
-__global__ void wait_flags_kernel(volatile unsigned int* flags, int n, unsigned int seq, uint32_t* status,
+static __global__ void wait_flags_kernel(volatile unsigned int* flags, int n, unsigned int seq, uint32_t* status,
                                   unsigned long long wait_limit_ns) {
   if (threadIdx.x >= n) return;
   const uint64_t t0 = ptx::globaltimer_ns();

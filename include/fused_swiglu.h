@@ -282,6 +282,39 @@ int fsw_route_backward(const void* logits, int64_t ld, const void* indices, cons
                        void* dlogits, int64_t T, int E, int k, int dtype, int score,
                        int renormalize, float scale, void* stream);
 
+/*
+ * Routed SwiGLU experts (mixture of experts; no counterpart in the reference):
+ *   y[t] = sum over j < k of weights[t, j] * (silu(x[t] @ w_gate[e]) * (x[t] @ w_up[e])) @ w_down[e],
+ *   e = indices[t, j].
+ * x (T, d), weights (T, k) of weights_dtype (FSW_FP32 or dtype), indices (T, k) int32,
+ * w_gate and w_up (E, d, f), w_down (E, f, d_out), y (T, d_out); d, f, d_out multiples of 8.
+ * A pair whose index is outside [0, E) contributes nothing; an index may repeat in a row.
+ *
+ * The caller gives the buffers.  With `saved` != NULL (saved_bytes of fsw_experts_sizes)
+ * the forward keeps there what fsw_experts_backward reads, and `scratch` needs
+ * forward_bytes; with saved == NULL it needs inference_bytes.  The backward's scratch needs
+ * backward_bytes.  Scratch means nothing after a call; calls that may overlap on the GPU
+ * need different buffers.
+ *
+ * fsw_experts_backward: any of dx (T, d), dweights (T, k), dw_gate, dw_up (both or neither)
+ * and dw_down may be NULL; all of an output is written (zeros for an expert without rows,
+ * and for the weight of a pair that was dropped).  Deterministic: no atomics.
+ */
+int fsw_experts_sizes(int64_t T, int k, int E, int64_t d, int64_t f, int64_t d_out,
+                      int64_t* saved_bytes, int64_t* forward_bytes, int64_t* inference_bytes,
+                      int64_t* backward_bytes);
+int fsw_experts_forward(const void* x, const void* weights, const void* indices,
+                        const void* w_gate, const void* w_up, const void* w_down, void* y,
+                        void* saved, int64_t saved_bytes, void* scratch, int64_t scratch_bytes,
+                        int64_t T, int k, int E, int64_t d, int64_t f, int64_t d_out, int dtype,
+                        int weights_dtype, void* stream);
+int fsw_experts_backward(const void* dy, const void* weights, const void* w_gate,
+                         const void* w_up, const void* w_down, const void* saved,
+                         int64_t saved_bytes, void* scratch, int64_t scratch_bytes, void* dx,
+                         void* dweights, void* dw_gate, void* dw_up, void* dw_down, int64_t T,
+                         int k, int E, int64_t d, int64_t f, int64_t d_out, int dtype,
+                         int weights_dtype, void* stream);
+
 /* Message for the last non-zero return on the calling thread ("" if none). */
 const char* fsw_last_error(void);
 
