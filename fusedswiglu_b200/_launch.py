@@ -412,3 +412,104 @@ def experts_backward(dy: torch.Tensor, weights: torch.Tensor, w_gate: torch.Tens
             ptr(dwd), T, k, E, d, f, d_out, _code(dy), _weights_code(weights, dy), _stream(dy))
     _lib.check("fsw_experts_backward", rc)
     return dx, dr, dwg, dwu, dwd
+
+
+def _blocks(n: int) -> int:
+    return -(-n // 128)
+
+
+@functools.lru_cache(maxsize=1024)
+def _fp8_scratch_bytes(name: str, *sizes: int) -> int:
+    n = int(getattr(_lib.load(), name)(*sizes))
+    if n < 0:
+        _lib.check(name, n)
+    return n
+
+
+def fp8_quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """q (T, d) e4m3 and scale (T, blocks), a view of block-major storage."""
+    code = _code(x)
+    _require_cuda(x)
+    T, d = x.shape
+    q = torch.empty((T, d), device=x.device, dtype=torch.float8_e4m3fn)
+    scale = torch.empty((_blocks(d), T), device=x.device, dtype=torch.float32)
+    with torch.cuda.device(x.device):
+        rc = _lib.load().fsw_fp8_quantize_rows(x.data_ptr(), q.data_ptr(), scale.data_ptr(), T, d, code, _stream(x))
+    _lib.check("fsw_fp8_quantize_rows", rc)
+    return q, scale.t()
+
+
+def fp8_quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """w (E, d_in, d_out) -> q (E, d_out, d_in) e4m3 and scale (E, blocks, blocks)."""
+    code = _code(w)
+    _require_cuda(w)
+    E, d_in, d_out = w.shape
+    q = torch.empty((E, d_out, d_in), device=w.device, dtype=torch.float8_e4m3fn)
+    scale = torch.empty((E, _blocks(d_out), _blocks(d_in)), device=w.device, dtype=torch.float32)
+    with torch.cuda.device(w.device):
+        rc = _lib.load().fsw_fp8_quantize_weight(w.data_ptr(), q.data_ptr(), scale.data_ptr(), E, d_in, d_out, code, _stream(w))
+    _lib.check("fsw_fp8_quantize_weight", rc)
+    return q, scale
+
+
+def fp8_gemm(xq: torch.Tensor, x_scale: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """y (T, N) in ``dtype``; the row scales may be strided."""
+    _require_cuda(xq, x_scale, q, scale)
+    T, K = xq.shape
+    y = torch.empty((T, q.shape[0]), device=xq.device, dtype=dtype)
+    code = _code(y)
+    with torch.cuda.device(xq.device):
+        rc = _lib.load().fsw_fp8_gemm(xq.data_ptr(), x_scale.data_ptr(), x_scale.stride(0), x_scale.stride(1), q.data_ptr(),
+                                      scale.data_ptr(), y.data_ptr(), T, K, q.shape[0], code, _stream(xq))
+    _lib.check("fsw_fp8_gemm", rc)
+    return y
+
+
+def fp8_linear(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """y (T, N) = x (T, K) times the quantised weight (N, K)."""
+    code = _code(x)
+    _require_cuda(x, q, scale)
+    T, K = x.shape
+    N = q.shape[0]
+    nbytes = _fp8_scratch_bytes("fsw_fp8_linear_scratch_bytes", T, K)
+    y = torch.empty((T, N), device=x.device, dtype=x.dtype)
+    scratch = _scratch(nbytes, x)
+    with torch.cuda.device(x.device):
+        rc = _lib.load().fsw_fp8_linear(x.data_ptr(), q.data_ptr(), scale.data_ptr(), y.data_ptr(), scratch.data_ptr(), nbytes,
+                                        T, K, N, code, _stream(x))
+    _lib.check("fsw_fp8_linear", rc)
+    return y
+
+
+def fp8_mlp(x: torch.Tensor, w_gate: torch.Tensor, s_gate: torch.Tensor, w_up: torch.Tensor, s_up: torch.Tensor,
+            w_down: torch.Tensor, s_down: torch.Tensor) -> torch.Tensor:
+    code = _code(x)
+    _require_cuda(x, w_gate, s_gate, w_up, s_up, w_down, s_down)
+    (T, d), (d_out, f) = x.shape, w_down.shape
+    nbytes = _fp8_scratch_bytes("fsw_fp8_mlp_scratch_bytes", T, d, f)
+    y = torch.empty((T, d_out), device=x.device, dtype=x.dtype)
+    scratch = _scratch(nbytes, x)
+    with torch.cuda.device(x.device):
+        rc = _lib.load().fsw_fp8_mlp(
+            x.data_ptr(), w_gate.data_ptr(), s_gate.data_ptr(), w_up.data_ptr(), s_up.data_ptr(), w_down.data_ptr(),
+            s_down.data_ptr(), y.data_ptr(), scratch.data_ptr(), nbytes, T, d, f, d_out, code, _stream(x))
+    _lib.check("fsw_fp8_mlp", rc)
+    return y
+
+
+def fp8_experts(x: torch.Tensor, weights: torch.Tensor, indices: torch.Tensor, w_gate: torch.Tensor, s_gate: torch.Tensor,
+                w_up: torch.Tensor, s_up: torch.Tensor, w_down: torch.Tensor, s_down: torch.Tensor) -> torch.Tensor:
+    code = _code(x)
+    _require_cuda(x, weights, indices, w_gate, s_gate, w_up, s_up, w_down, s_down)
+    (T, d), k = x.shape, weights.shape[1]
+    E, d_out, f = w_down.shape
+    nbytes = _fp8_scratch_bytes("fsw_fp8_experts_scratch_bytes", T, k, E, d, f, d_out)
+    y = torch.empty((T, d_out), device=x.device, dtype=x.dtype)
+    scratch = _scratch(nbytes, x)
+    with torch.cuda.device(x.device):
+        rc = _lib.load().fsw_fp8_experts_forward(
+            x.data_ptr(), weights.data_ptr(), indices.data_ptr(), w_gate.data_ptr(), s_gate.data_ptr(), w_up.data_ptr(),
+            s_up.data_ptr(), w_down.data_ptr(), s_down.data_ptr(), y.data_ptr(), scratch.data_ptr(), nbytes, T, k, E, d, f,
+            d_out, code, _weights_code(weights, x), _stream(x))
+    _lib.check("fsw_fp8_experts_forward", rc)
+    return y

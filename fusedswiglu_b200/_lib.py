@@ -45,6 +45,15 @@ SIGNATURES = {
     "fsw_experts_sizes": (c_int, [c_int64, c_int, c_int] + [c_int64] * 3 + [POINTER(c_int64)] * 4),
     "fsw_experts_forward": (c_int, [c_void_p] * 8 + [c_int64, c_void_p, c_int64, c_int64, c_int, c_int] + [c_int64] * 3 + [c_int, c_int, c_void_p]),
     "fsw_experts_backward": (c_int, [c_void_p] * 6 + [c_int64, c_void_p, c_int64] + [c_void_p] * 5 + [c_int64, c_int, c_int] + [c_int64] * 3 + [c_int, c_int, c_void_p]),
+    "fsw_fp8_quantize_rows": (c_int, [c_void_p] * 3 + [c_int64] * 2 + [c_int, c_void_p]),
+    "fsw_fp8_quantize_weight": (c_int, [c_void_p] * 3 + [c_int, c_int64, c_int64, c_int, c_void_p]),
+    "fsw_fp8_gemm": (c_int, [c_void_p] * 2 + [c_int64] * 2 + [c_void_p] * 3 + [c_int64] * 3 + [c_int, c_void_p]),
+    "fsw_fp8_linear_scratch_bytes": (c_int64, [c_int64] * 2),
+    "fsw_fp8_linear": (c_int, [c_void_p] * 5 + [c_int64] * 4 + [c_int, c_void_p]),
+    "fsw_fp8_mlp_scratch_bytes": (c_int64, [c_int64] * 3),
+    "fsw_fp8_mlp": (c_int, [c_void_p] * 9 + [c_int64] * 5 + [c_int, c_void_p]),
+    "fsw_fp8_experts_scratch_bytes": (c_int64, [c_int64, c_int, c_int] + [c_int64] * 3),
+    "fsw_fp8_experts_forward": (c_int, [c_void_p] * 11 + [c_int64, c_int64, c_int, c_int] + [c_int64] * 3 + [c_int, c_int, c_void_p]),
     "fsw_last_error": (c_char_p, []),
     "fsw_query_device": (c_int, [c_int, POINTER(c_int), POINTER(c_int), POINTER(c_int), POINTER(c_int64)]),
     "fsw_status": (c_int64, []),

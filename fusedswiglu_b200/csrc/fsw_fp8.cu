@@ -1,0 +1,887 @@
+// Products in 8-bit floating point (e4m3) with a scale for each block of 128:
+//
+//   y[t, n] = sum over b of xs[t, b] * ws[n / 128, b] * sum over k in block b of xq[t, k] wq[n, k]
+//
+// and the SwiGLU gate on top of two of them, with its result quantised again:
+//   h = silu(x Wg) * (x Wu),  hs[t, b] = 2^e with the smallest e that makes the largest |h| of
+//   the block at most 448,  hq = round(h / hs).
+// Activations have one scale per row and 128 columns, weights one per 128 x 128.  Activation
+// scales made here are powers of two: dividing by them is exact, so a value is rounded once;
+// the weights' scales may be any fp32 numbers.
+//
+// The tensor cores add the 128 products of a block in tensor memory (kind::f8f6f4, fp32);
+// the blocks' sums are scaled and added in fp32 registers by the epilogue warps, beside the
+// MMAs of the next block.  A tile is 128 tokens x 256 weight rows per CTA (256 x 256 per CTA
+// pair); in 512 cycles of MMAs per block and pair the epilogue reads 128 x 256 sums per SM
+// from tensor memory (256 cycles) and issues 128 packed FMAs per scheduler.
+//
+// Few rows: the A box holds only the rows there are, and with fewer tiles than SMs the K
+// blocks of a tile are divided over the CTAs of a cluster, which add their sums through
+// distributed shared memory in a fixed order.
+#include <cuda_fp8.h>
+
+#include <cstring>
+
+#include "fsw_experts.h"
+#include "fsw_gemm.cuh"
+
+namespace fsw {
+namespace {
+
+constexpr int kBlock = 128;
+constexpr float kE4M3Max = 448.0f;
+
+struct Fp8Params {
+  CUtensorMap a, b0, b1;
+  uint64_t desc;
+  uint32_t idesc;
+  const float* xs;          // xs[row * xs_row + block * xs_block]
+  int64_t xs_row, xs_block;
+  const float *ws0, *ws1;   // (E, row blocks, K blocks)
+  int ws_rows, num_kb;
+  int M, N;                 // output rows and columns
+  int num_m_tiles, num_n_tiles, group_m;
+  void* out;                // (M, N) of the output type
+  uint8_t* hq;              // dual: (M, N) e4m3
+  float* hs;                // dual: hs[block * hs_pitch + row]
+  int64_t hs_pitch;
+  const int *grp_meta, *grp_tile_expert, *grp_offsets, *grp_counts;  // grp_meta nullptr: one weight
+  int a_rows;               // rows of an A box
+  int splits;               // CTAs of a cluster that share a tile's K blocks (CG == 1, one tile each)
+  uint32_t* status;
+  unsigned long long wait_limit_ns;
+  int stall_producer;
+};
+
+template <int CG>
+struct Fp8Cfg {
+  static constexpr int A_BYTES = 128 * kBlock;
+  static constexpr int B_BYTES = 256 / CG * kBlock;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = CG == 2 ? 6 : 4;
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int EPI_BUF_BYTES = 32 * 128;
+  static constexpr int BAR_BYTES = 512;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * EPI_BUF_BYTES + BAR_BYTES + 1024;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static_assert(SMEM_BYTES <= kSmemBudget, "shared memory");
+  // a split tile's sums overlay the operand stages: 8 warps x 128 columns x 32 lanes
+  static_assert(EPI_WARPS * 128 * 32 * 4 <= STAGES * STAGE_BYTES, "partial sums");
+};
+
+template <int CG>
+__device__ __forceinline__ void mma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Completes the loads in flight; the registers pass through it, so that no use moves ahead.
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+// acc[0..15] += s * t[0..15], as packed pairs.
+__device__ __forceinline__ void scaled_add16(float* acc, const uint32_t (&t)[16], float s) {
+  unsigned long long s2;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(s));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    unsigned long long t2, a2;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(t2) : "r"(t[2 * i]), "r"(t[2 * i + 1]));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(a2) : "f"(acc[2 * i]), "f"(acc[2 * i + 1]));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a2) : "l"(t2), "l"(s2));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[2 * i]), "=f"(acc[2 * i + 1]) : "l"(a2));
+  }
+}
+
+// Scale of a block whose largest magnitude has these bits: the smallest power of two 2^e with
+// amax <= 448 * 2^e (448 = 1.75 * 2^8), at least 2^-126; 1 for a block of zeros; NaN if the
+// block holds inf or NaN (its products are then NaN).  `inv` is the exact inverse.
+__device__ __forceinline__ float block_scale(uint32_t amax_bits, float& inv) {
+  if (amax_bits == 0u) {
+    inv = 1.0f;
+    return 1.0f;
+  }
+  if (amax_bits >= 0x7f800000u) {
+    inv = 1.0f;
+    return __uint_as_float(0x7fc00000u);
+  }
+  int e = static_cast<int>(amax_bits >> 23) - ((amax_bits & 0x7fffffu) <= 0x600000u ? 8 : 7);  // biased exponent
+  if (e < 1) e = 1;
+  inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+  return __uint_as_float(static_cast<uint32_t>(e) << 23);
+}
+__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+struct Fp8Work {
+  int m_tile, n_tile, expert, rows;  // rows: valid rows from the tile's first on
+};
+
+// --------------------------------------------------------------------- GEMM --
+template <int CG, bool DUAL, typename T>
+__global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const __grid_constant__ Fp8Params p) {
+  using C = Fp8Cfg<CG>;
+  constexpr int STAGES = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_u32 = ptx::smem_u32(smem_raw);
+  const uint32_t smem_base = (raw_u32 + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - raw_u32);
+  const uint32_t epi_base = smem_base + STAGES * C::STAGE_BYTES;
+  const uint32_t amax_off = STAGES * C::STAGE_BYTES;  // DUAL: in place of the store buffers
+  const uint32_t bar_base = epi_base + C::EPI_WARPS * C::EPI_BUF_BYTES;
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+  auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
+  auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + 2 + a); };
+  const uint32_t misc_off = (bar_base - smem_base) + 8u * (2 * STAGES + 4);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_gen + misc_off);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem_gen + misc_off + 4);
+  const AbortCtl ctl{abort_flag, p.status, p.wait_limit_ns ? p.wait_limit_ns : kWaitLimitNs};
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = (CG == 2 || p.splits > 1) ? ptx::cluster_ctarank() : 0u;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(tfull_bar(a), 1);
+      ptx::mbar_init(tempty_bar(a), C::EPI_WARPS * CG);
+    }
+    *abort_flag = 0u;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    ptx::prefetch_tensormap(&p.a);
+    ptx::prefetch_tensormap(&p.b0);
+    if (DUAL) ptx::prefetch_tensormap(&p.b1);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc<CG>(bar_base + 8u * (2 * STAGES + 4), 512);
+    ptx::tmem_relinquish<CG>();
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (CG == 2) {
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+  }
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int cluster = CG * p.splits;
+  const int num_clusters = gridDim.x / cluster, cluster_id = blockIdx.x / cluster;
+  const int m_tiles = p.grp_meta != nullptr ? p.grp_meta[0] : p.num_m_tiles;
+  // this CTA's share of a tile's K blocks
+  const int share = p.splits > 1 ? static_cast<int>(rank) : 0;
+  const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * share / p.splits);
+  const int kb1 = static_cast<int>(static_cast<long long>(p.num_kb) * (share + 1) / p.splits);
+  auto get_work = [&](int idx, Fp8Work& w) {
+    const long long t = cluster_id + static_cast<long long>(idx) * num_clusters;
+    if (t >= static_cast<long long>(m_tiles) * p.num_n_tiles) return false;
+    decode_tile_order(static_cast<int>(t), m_tiles, p.num_n_tiles, p.group_m, w.m_tile, w.n_tile);
+    const int row0 = w.m_tile * 128 * CG;
+    if (p.grp_meta != nullptr) {
+      w.expert = p.grp_tile_expert[w.m_tile];
+      w.rows = p.grp_offsets[w.expert] + p.grp_counts[w.expert] - row0;
+    } else {
+      w.expert = 0;
+      w.rows = p.M - row0;
+    }
+    return true;
+  };
+
+  if (warp == 0) {
+    // ======================= TMA producer (one thread) =======================
+    if (lane == 0 && !p.stall_producer) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      const uint64_t pol = ptx::make_l2_policy(2);
+      const uint32_t bytes = CG * (static_cast<uint32_t>(p.a_rows) * kBlock + C::B_BYTES);
+      Fp8Work w;
+      for (int idx = 0; ok && get_work(idx, w); ++idx) {
+        const int m0 = w.m_tile * 128 * CG + (CG == 2 ? rank * 128 : 0);
+        const int n0 = w.n_tile * (DUAL ? 128 : 256);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = bounded_wait_thread(empty_bar(s), ph ^ 1u, ctl, WAIT_PRODUCER_EMPTY);
+          if (!ok) break;
+          const uint32_t a_dst = smem_base + s * C::STAGE_BYTES, b_dst = a_dst + C::A_BYTES;
+          uint32_t fb = full_bar(s);
+          if (CG == 2) fb = ptx::mapa(fb, 0);
+          if (CG == 1 || rank == 0) ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
+          const int k0 = kb * kBlock;
+          if constexpr (CG == 2) {
+            ptx::tma_load_2d_pair(a_dst, &p.a, fb, k0, m0, pol);
+            if (DUAL)
+              ptx::tma_load_3d_pair(b_dst, rank ? &p.b1 : &p.b0, fb, k0, n0, w.expert, pol);
+            else
+              ptx::tma_load_3d_pair(b_dst, &p.b0, fb, k0, n0 + static_cast<int>(rank) * 128, w.expert, pol);
+          } else {
+            ptx::tma_load_2d(a_dst, &p.a, fb, k0, m0, pol);
+            ptx::tma_load_3d(b_dst, &p.b0, fb, k0, n0, w.expert, pol);
+            ptx::tma_load_3d(b_dst + 128 * kBlock, DUAL ? &p.b1 : &p.b0, fb, k0, DUAL ? n0 : n0 + 128, w.expert, pol);
+          }
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ================ MMA issuer (one thread of the pair leader) ================
+    if ((CG == 1 || rank == 0) && lane == 0) {
+      int s = 0, a = 0;
+      uint32_t ph = 0, aph = 0;
+      bool ok = true;
+      auto commit = [&](uint32_t bar) {
+        if (CG == 2)
+          ptx::mma_commit_pair(bar, 3);
+        else
+          ptx::mma_commit(bar);
+      };
+      Fp8Work w;
+      for (int idx = 0; ok && get_work(idx, w); ++idx) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = bounded_wait_thread(full_bar(s), ph, ctl, WAIT_MMA_FULL);
+          if (ok) ok = bounded_wait_thread(tempty_bar(a), aph ^ 1u, ctl, WAIT_MMA_TMEM_EMPTY);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          const uint32_t a_addr = smem_base + s * C::STAGE_BYTES, b_addr = a_addr + C::A_BYTES;
+#pragma unroll
+          for (int k = 0; k < kBlock / 32; ++k)
+            mma_f8_ss<CG>(tmem_base + a * 256, p.desc | (((a_addr + k * 32u) & 0x3FFFFu) >> 4),
+                          p.desc | (((b_addr + k * 32u) & 0x3FFFFu) >> 4), p.idesc, k != 0 ? 1u : 0u);
+          commit(empty_bar(s));
+          commit(tfull_bar(a));
+          a ^= 1;
+          if (a == 0) aph ^= 1u;
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+  } else {
+    // ======================= epilogue: scale, add, write =======================
+    const int q = warp & 3, ew = warp - 2, half = ew >> 2;
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+    // Columns of this warp within a region: one weight block of 128, or, with two weights, the
+    // same 64 columns of both, so that a thread holds gate and up of its columns.
+    const uint32_t col_lo = DUAL ? half * 64 : half * 128;
+    const uint32_t col_hi = DUAL ? 128 + half * 64 : half * 128 + 64;
+    const uint32_t buf = epi_base + ew * C::EPI_BUF_BYTES;
+    int a = 0;
+    uint32_t aph = 0;
+    bool ok = true;
+    int parity = 0;
+    Fp8Work w;
+    for (int idx = 0; ok && get_work(idx, w); ++idx) {
+      const int tile_row = (CG == 2 ? static_cast<int>(rank) * 128 : 0) + q * 32;  // of this warp, in the tile
+      const int row0 = w.m_tile * 128 * CG + tile_row;
+      const bool active = tile_row < w.rows;  // no valid row here: nothing is added up or stored
+      const int row = row0 + lane < p.M ? row0 + lane : p.M - 1;
+      const int nb = DUAL ? w.n_tile : 2 * w.n_tile + half;
+      const bool have_block = nb < p.ws_rows;
+      const int64_t wbase = (static_cast<int64_t>(w.expert) * p.ws_rows + (have_block ? nb : 0)) * p.num_kb;
+      const float* xs = p.xs + static_cast<int64_t>(row) * p.xs_row;
+      float acc[128];
+#pragma unroll
+      for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+      float x_next = 0.0f, lo_next = 0.0f, hi_next = 0.0f;
+      auto fetch = [&](int kb) {
+        if (active && kb < kb1) {
+          x_next = xs[kb * p.xs_block];
+          lo_next = p.ws0[wbase + kb];
+          hi_next = DUAL ? p.ws1[wbase + kb] : lo_next;
+        }
+      };
+      fetch(kb0);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const float s_lo = x_next * lo_next, s_hi = x_next * hi_next;
+        fetch(kb + 1);
+        ok = bounded_wait_warp(tfull_bar(a), aph, ctl, WAIT_EPI_TMEM_FULL);
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        auto release = [&]() {
+          ptx::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            if (CG == 2)
+              ptx::mbar_arrive_cluster(ptx::mapa(tempty_bar(a), 0));
+            else
+              ptx::mbar_arrive(tempty_bar(a));
+          }
+        };
+        if (active) {
+          // eight chunks of 16 columns, two loads in flight
+          const uint32_t t0 = lane_base + a * 256;
+          uint32_t r0[16], r1[16];
+          ptx::tmem_ld_32x16(t0 + col_lo, r0);
+#pragma unroll
+          for (int c = 0; c < 8; c += 2) {
+            tmem_wait16(r0);
+            ptx::tmem_ld_32x16(t0 + (c + 1 < 4 ? col_lo + (c + 1) * 16 : col_hi + (c - 3) * 16), r1);
+            scaled_add16(acc + c * 16, r0, c < 4 ? s_lo : s_hi);
+            tmem_wait16(r1);
+            if (c + 2 < 8)
+              ptx::tmem_ld_32x16(t0 + (c + 2 < 4 ? col_lo + (c + 2) * 16 : col_hi + (c - 2) * 16), r0);
+            else
+              release();
+            scaled_add16(acc + (c + 1) * 16, r1, c + 1 < 4 ? s_lo : s_hi);
+          }
+        } else {
+          release();
+        }
+        a ^= 1;
+        if (a == 0) aph ^= 1u;
+      }
+      // The two warps of a lane quadrant meet once a tile (below).  One that gives up arrives
+      // there without waiting, and none waits once the flag is up: no warp is left behind.
+      if (DUAL && ok) ok = __all_sync(0xffffffffu, *abort_flag == 0u);
+      if (!ok) {
+        if (DUAL) asm volatile("bar.arrive %0, 64;" ::"r"(1 + q) : "memory");
+        break;
+      }
+
+      if (!DUAL && p.splits > 1) {
+        // partial sums of this share, [warp][column][lane]; added up behind the cluster barrier.
+        // Every MMA and load of this CTA is complete: the stages are free.
+        if (active) {
+          float* part = reinterpret_cast<float*>(smem_gen) + ew * 128 * 32 + lane;
+#pragma unroll
+          for (int i = 0; i < 128; ++i) part[i * 32] = acc[i];
+        }
+      } else if constexpr (!DUAL) {
+        if (active) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) pk[i] = pack2<T>(acc[j * 64 + 2 * i], acc[j * 64 + 2 * i + 1]);
+            stage_rows128(buf, lane, pk);
+            __syncwarp();
+            flush_rows128(buf, lane, p.out, row0, w.n_tile * 256 + half * 128 + j * 64, p.M, p.N, p.N);
+            __syncwarp();
+          }
+        }
+      } else {
+        // h = silu(g) u in fp32; the row's block of 128 columns is shared by the two warps of
+        // this lane quadrant, which exchange their largest magnitudes
+        uint32_t top = 0u;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+          const float g = acc[i];
+          acc[i] = g * sigmoid_f32(g) * acc[64 + i];
+          const uint32_t m = magnitude_bits(acc[i]);
+          top = top > m ? top : m;
+        }
+        volatile uint32_t* mine = reinterpret_cast<volatile uint32_t*>(smem_gen + amax_off) + (parity * C::EPI_WARPS) * 32;
+        mine[ew * 32 + lane] = top;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
+        const uint32_t other = mine[(ew ^ 4) * 32 + lane];
+        parity ^= 1;
+        float inv;
+        const float scale = block_scale(top > other ? top : other, inv);
+        if (active && row0 + lane < p.M) {
+          if (half == 0) p.hs[w.n_tile * p.hs_pitch + row0 + lane] = scale;
+          uint8_t* dst = p.hq + static_cast<int64_t>(row0 + lane) * p.N;
+          const int col = w.n_tile * 128 + half * 64;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float* h = acc + c * 16 + i * 4;
+              v[i] = to_e4m3x4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
+            }
+            if (col + c * 16 < p.N) ptx::st_global_v4(dst + col + c * 16, v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+    }
+  }
+
+  // ======================= shares of one tile, teardown =======================
+  __syncwarp();
+  if (CG == 1 && !DUAL && p.splits > 1) {
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+    Fp8Work w;
+    if (warp >= 2 && get_work(0, w)) {
+      const int q = warp & 3, ew = warp - 2, half = ew >> 2;
+      const int row = w.m_tile * 128 + q * 32 + lane;
+      if (q * 32 < w.rows) {
+        // this CTA adds and writes columns [rank * per, (rank + 1) * per) of each warp's 128
+        const int per = 128 / p.splits;
+        for (int c0 = static_cast<int>(rank) * per; c0 < (static_cast<int>(rank) + 1) * per; c0 += 8) {
+          float sum[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
+          for (int r = 0; r < p.splits; ++r) {
+            const uint32_t base = ptx::mapa(smem_base + ((ew * 128 + c0) * 32 + lane) * 4u, r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += ld_cluster_f32(base + i * 128u);
+          }
+          const int col = w.n_tile * 256 + half * 128 + c0;
+          if (row < p.M && col < p.N && *abort_flag == 0u)
+            ptx::st_global_v4(static_cast<T*>(p.out) + static_cast<int64_t>(row) * p.N + col, pack2<T>(sum[0], sum[1]),
+                              pack2<T>(sum[2], sum[3]), pack2<T>(sum[4], sum[5]), pack2<T>(sum[6], sum[7]));
+        }
+      }
+    }
+    __syncwarp();
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag != 0u) {
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < kDrainNs) __nanosleep(1000);
+  }
+  if (CG == 2 || p.splits > 1) {
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+  }
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc<CG>(tmem_base, 512);
+  }
+}
+
+// ------------------------------------------------------------- quantisation --
+template <typename T>
+__device__ __forceinline__ void load8(const T* src, float (&v)[8]) {
+  const uint4 x = *reinterpret_cast<const uint4*>(src);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
+}
+
+// One token per block row; 16 lanes take the 8-element pieces of a block of 128 columns.
+// With a plan the token's row goes to the rows of its k pairs.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
+                                                            float* __restrict__ scales, int64_t pitch, int d,
+                                                            const ExpertPlan plan, const int* __restrict__ plan_dev) {
+  const int64_t t = blockIdx.x;
+  const int k = plan_dev != nullptr ? plan.k : 1;
+  for (int c0 = (blockIdx.y * 256 + threadIdx.x) * 8; c0 - static_cast<int>(threadIdx.x & 15) * 8 < d; c0 += gridDim.y * 256 * 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    if (c0 < d) load8<T>(x + t * d + c0, v);
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, magnitude_bits(v[i]));
+    const unsigned half_mask = 0xffffu << (threadIdx.x & 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(half_mask, top, o));
+    float inv;
+    const float scale = block_scale(top, inv);
+    const uint2 packed = make_uint2(to_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                                    to_e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+    for (int j = 0; j < k; ++j) {
+      const int64_t row = plan_dev != nullptr ? plan_dev[plan.pair_row + t * k + j] : t;
+      if (row < 0) continue;
+      if (c0 < d) *reinterpret_cast<uint2*>(q + row * d + c0) = packed;
+      if ((threadIdx.x & 15) == 0) scales[(c0 >> 7) * pitch + row] = scale;
+    }
+  }
+}
+
+// w (d_in, d_out) -> q (d_out, d_in) and a power-of-two scale per 128 x 128 block.
+// One block of threads per block of the weight; runs once per weight.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_weight_kernel(const T* __restrict__ w, uint8_t* __restrict__ q,
+                                                              float* __restrict__ scales, int d_in, int d_out) {
+  __shared__ __align__(16) uint8_t tile[128][132];
+  __shared__ uint32_t tops[8];
+  const int64_t e = blockIdx.z;
+  const int k0 = blockIdx.x * 128, n0 = blockIdx.y * 128;
+  const T* src = w + e * d_in * d_out;
+  uint32_t top = 0u;
+  float v[8][8];
+  const int piece = threadIdx.x & 15;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int kk = k0 + i * 16 + (threadIdx.x >> 4), n = n0 + piece * 8;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v[i][c] = 0.0f;
+    if (kk < d_in && n < d_out) load8<T>(src + static_cast<int64_t>(kk) * d_out + n, v[i]);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) top = max(top, magnitude_bits(v[i][c]));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, tops[i]);
+  float inv;
+  const float scale = block_scale(top, inv);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int c = 0; c < 8; c += 4) {
+      const uint32_t b = to_e4m3x4(v[i][c] * inv, v[i][c + 1] * inv, v[i][c + 2] * inv, v[i][c + 3] * inv);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tile[piece * 8 + c + j][i * 16 + (threadIdx.x >> 4)] = static_cast<uint8_t>(b >> (8 * j));
+    }
+  if (threadIdx.x == 0) scales[(e * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = scale;
+  __syncthreads();
+  for (int i = threadIdx.x; i < 128 * 32; i += 256) {
+    const int n = i >> 5, kk = (i & 31) * 4;
+    if (n0 + n < d_out && k0 + kk < d_in)
+      *reinterpret_cast<uint32_t*>(q + (e * d_out + n0 + n) * static_cast<int64_t>(d_in) + k0 + kk) =
+          *reinterpret_cast<const uint32_t*>(&tile[n][kk]);
+  }
+}
+
+// ------------------------------------------------------------------ launches --
+template <int CG, bool DUAL, typename T>
+int launch_fp8_one(const Fp8Params& p, int grid, cudaStream_t st) {
+  static std::atomic<uint64_t> prepared{0};
+  int dev = 0;
+  FSW_CUDA(cudaGetDevice(&dev));
+  if (!(prepared.load() >> (dev & 63) & 1)) {
+    FSW_CUDA(cudaFuncSetAttribute(fp8_gemm_kernel<CG, DUAL, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  Fp8Cfg<CG>::SMEM_BYTES));
+    prepared.fetch_or(1ull << (dev & 63));
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(Fp8Cfg<CG>::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = Fp8Cfg<CG>::SMEM_BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG * p.splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  ++g_kernel_launches;
+  FSW_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<CG, DUAL, T>, p));
+  return FSW_OK;
+}
+
+// The rows an 8-bit product works on: T dense rows, or a plan's.
+struct Fp8Rows {
+  int64_t rows;                 // of the arrays
+  int64_t most;                 // most rows a weight can have
+  const ExpertPlan* plan;       // nullptr: dense
+  const int* plan_dev;
+};
+
+// out (rows, N) = x @ w^T, or with w1 hq, hs = quantised silu(x w^T) * (x w1^T).
+int run_fp8(const Fp8Rows& r, const void* xq, const float* xs, int64_t xs_row, int64_t xs_block, const void* w,
+            const float* ws, const void* w1, const float* ws1, void* out, uint8_t* hq, float* hs, int64_t K, int64_t N,
+            int dtype, DeviceInfo* d, cudaStream_t st) {
+  const bool dual = w1 != nullptr;
+  const int E = r.plan != nullptr ? r.plan->E : 1;
+  const int tile_n = dual ? 128 : 256;
+  Fp8Params p;
+  memset(&p, 0, sizeof(p));
+  p.num_kb = (int)((K + kBlock - 1) / kBlock);
+  p.num_n_tiles = (int)((N + tile_n - 1) / tile_n);
+  p.ws_rows = (int)((N + kBlock - 1) / kBlock);
+  // Pairs of CTAs halve the operand traffic of a tile; a single CTA's tile fits fewer rows.
+  int cg;
+  if (r.plan != nullptr)
+    cg = r.plan->tile_rows / 128;
+  else
+    cg = (r.rows + 255) / 256 * p.num_n_tiles >= d->max_pairs / 2 && r.rows > 128 ? 2 : 1;
+  p.num_m_tiles = r.plan != nullptr ? r.plan->tiles : (int)((r.rows + 128 * cg - 1) / (128 * cg));
+  const long long tiles = (long long)p.num_m_tiles * p.num_n_tiles;
+  if (tiles >= (1ll << 30)) return fail(FSW_EINVAL, "too many tiles");
+  p.splits = 1;
+  if (cg == 1 && !dual && r.plan == nullptr) {
+    // fewer tiles than half the SMs: divide their K blocks, at least 4 blocks a share
+    while (p.splits < 8 && tiles * p.splits * 2 <= d->sm_count && p.num_kb >= 8 * p.splits) p.splits *= 2;
+  }
+  p.a_rows = r.most > 120 ? 128 : (int)((r.most + 7) / 8 * 8);
+  if (cg == 2) p.a_rows = 128;
+  int rc;
+  if ((rc = make_map(&p.a, xq, 0, K, r.rows, p.a_rows, "x", 128, 0, 0, 1)) != FSW_OK) return rc;
+  if ((rc = make_map(&p.b0, w, 0, K, N, 128, "weight", 128, 0, E, 1)) != FSW_OK) return rc;
+  p.b1 = p.b0;
+  if (dual && (rc = make_map(&p.b1, w1, 0, K, N, 128, "w_up", 128, 0, E, 1)) != FSW_OK) return rc;
+  uint32_t kadv;
+  fill_operand_desc(MAJOR_K, &p.desc, &kadv);
+  // kind::f8f6f4: fp32 sums (bit 4), e4m3 operands (0), both K-major
+  p.idesc = (1u << 4) | (256u >> 3 << 17) | (static_cast<uint32_t>(128 * cg) >> 4 << 24);
+  p.xs = xs;
+  p.xs_row = xs_row;
+  p.xs_block = xs_block;
+  p.ws0 = ws;
+  p.ws1 = ws1;
+  p.M = (int)r.rows;
+  p.N = (int)N;
+  p.out = out;
+  p.hq = hq;
+  p.hs = hs;
+  p.hs_pitch = r.rows;
+  if (r.plan != nullptr) {
+    p.grp_meta = r.plan_dev;
+    p.grp_counts = r.plan_dev + r.plan->counts;
+    p.grp_offsets = r.plan_dev + r.plan->offsets;
+    p.grp_tile_expert = r.plan_dev + r.plan->tile_expert;
+  }
+  p.status = d->status;
+  p.wait_limit_ns = (unsigned long long)opt_wait_limit_ms() * 1000000ull;
+  p.stall_producer = (int)opt_stall_producer();
+  p.group_m = p.num_m_tiles < 8 ? p.num_m_tiles : 8;
+  const long long workers = cg == 2 ? d->max_pairs : d->sm_count;
+  const int grid = (int)(p.splits > 1 ? tiles * p.splits : (tiles < workers ? tiles : workers) * cg);
+  const bool bf = dtype == FSW_BF16;
+  if (cg == 2) {
+    if (dual) return launch_fp8_one<2, true, __nv_bfloat16>(p, grid, st);
+    return bf ? launch_fp8_one<2, false, __nv_bfloat16>(p, grid, st) : launch_fp8_one<2, false, __half>(p, grid, st);
+  }
+  if (dual) return launch_fp8_one<1, true, __nv_bfloat16>(p, grid, st);
+  return bf ? launch_fp8_one<1, false, __nv_bfloat16>(p, grid, st) : launch_fp8_one<1, false, __half>(p, grid, st);
+}
+
+int quantize_rows(const void* x, void* q, float* scales, int64_t pitch, int64_t T, int64_t d, int dtype,
+                  const ExpertPlan* plan, const int* plan_dev, cudaStream_t st) {
+  ExpertPlan none = {};
+  // a block covers 2048 columns; few tokens are spread over more blocks
+  const dim3 grid((unsigned)T, (unsigned)(T >= 1024 ? 1 : (d + 2047) / 2048));
+  ++g_kernel_launches;
+  if (dtype == FSW_BF16)
+    quantize_rows_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(x), static_cast<uint8_t*>(q),
+                                                              scales, pitch, (int)d, plan ? *plan : none, plan_dev);
+  else
+    quantize_rows_kernel<__half><<<grid, 256, 0, st>>>(static_cast<const __half*>(x), static_cast<uint8_t*>(q), scales,
+                                                       pitch, (int)d, plan ? *plan : none, plan_dev);
+  FSW_CUDA(cudaGetLastError());
+  return FSW_OK;
+}
+
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+int64_t blocks_of(int64_t v) { return (v + kBlock - 1) / kBlock; }
+
+int check_fp8(int64_t T, int64_t K, int64_t N, int dtype) {
+  if (dtype != FSW_BF16 && dtype != FSW_FP16) return fail(FSW_EINVAL, "unknown dtype %d", dtype);
+  if (T < 0 || T >= (1ll << 31) - 256) return fail(FSW_EINVAL, "bad number of rows %lld", (long long)T);
+  if (K <= 0 || N <= 0 || K >= (1 << 24) || N >= (1 << 24))
+    return fail(FSW_EINVAL, "bad feature sizes %lld, %lld", (long long)K, (long long)N);
+  if ((K & 15) || (N & 7))
+    return fail(FSW_EINVAL, "the inner size %lld must be a multiple of 16 and the outer size %lld of 8", (long long)K, (long long)N);
+  return FSW_OK;
+}
+
+}  // namespace
+}  // namespace fsw
+
+using namespace fsw;
+
+extern "C" {
+
+int fsw_fp8_quantize_rows(const void* x, void* q, void* scales, int64_t T, int64_t d, int dtype, void* stream) {
+  int rc = check_fp8(T, d, 8, dtype);
+  if (rc != FSW_OK) return rc;
+  if (T == 0) return FSW_OK;
+  if (!x || !q || !scales) return fail(FSW_EINVAL, "NULL pointer");
+  if (!aligned16(x) || !aligned16(q)) return fail(FSW_EINVAL, "pointers must be 16-byte aligned");
+  DeviceInfo* dev = nullptr;
+  if ((rc = ensure_device(&dev)) != FSW_OK) return rc;
+  return quantize_rows(x, q, static_cast<float*>(scales), T, T, d, dtype, nullptr, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+int fsw_fp8_quantize_weight(const void* w, void* q, void* scales, int E, int64_t d_in, int64_t d_out, int dtype, void* stream) {
+  int rc = check_fp8(1, d_in, d_out, dtype);
+  if (rc != FSW_OK) return rc;
+  if (E < 1 || E > FSW_MAX_EXPERTS || blocks_of(d_out) > 65535) return fail(FSW_EINVAL, "bad number of weights %d or size", E);
+  if (!w || !q || !scales) return fail(FSW_EINVAL, "NULL pointer");
+  if (!aligned16(w) || !aligned16(q)) return fail(FSW_EINVAL, "pointers must be 16-byte aligned");
+  DeviceInfo* dev = nullptr;
+  if ((rc = ensure_device(&dev)) != FSW_OK) return rc;
+  const dim3 grid((unsigned)blocks_of(d_in), (unsigned)blocks_of(d_out), (unsigned)E);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ++g_kernel_launches;
+  if (dtype == FSW_BF16)
+    quantize_weight_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(w), static_cast<uint8_t*>(q),
+                                                                static_cast<float*>(scales), (int)d_in, (int)d_out);
+  else
+    quantize_weight_kernel<__half><<<grid, 256, 0, st>>>(static_cast<const __half*>(w), static_cast<uint8_t*>(q),
+                                                         static_cast<float*>(scales), (int)d_in, (int)d_out);
+  FSW_CUDA(cudaGetLastError());
+  return FSW_OK;
+}
+
+int fsw_fp8_gemm(const void* xq, const void* xs, int64_t xs_row_stride, int64_t xs_block_stride, const void* w,
+                 const void* ws, void* y, int64_t T, int64_t K, int64_t N, int dtype, void* stream) {
+  int rc = check_fp8(T, K, N, dtype);
+  if (rc != FSW_OK) return rc;
+  if (xs_row_stride < 0 || xs_block_stride < 0) return fail(FSW_EINVAL, "negative stride of the scales");
+  if (T == 0) return FSW_OK;
+  if (!xq || !xs || !w || !ws || !y) return fail(FSW_EINVAL, "NULL pointer");
+  if (!aligned16(xq) || !aligned16(w) || !aligned16(y)) return fail(FSW_EINVAL, "pointers must be 16-byte aligned");
+  DeviceInfo* dev = nullptr;
+  if ((rc = ensure_device(&dev)) != FSW_OK) return rc;
+  const Fp8Rows r = {T, T, nullptr, nullptr};
+  return run_fp8(r, xq, static_cast<const float*>(xs), xs_row_stride, xs_block_stride, w, static_cast<const float*>(ws),
+                 nullptr, nullptr, y, nullptr, nullptr, K, N, dtype, dev, static_cast<cudaStream_t>(stream));
+}
+
+int64_t fsw_fp8_linear_scratch_bytes(int64_t T, int64_t K) {
+  int rc = check_fp8(T, K, 8, FSW_BF16);
+  if (rc != FSW_OK) return rc;
+  return align256(T * K) + align256(T * blocks_of(K) * 4);
+}
+
+int fsw_fp8_linear(const void* x, const void* w, const void* ws, void* y, void* scratch, int64_t scratch_bytes, int64_t T,
+                   int64_t K, int64_t N, int dtype, void* stream) {
+  int rc = check_fp8(T, K, N, dtype);
+  if (rc != FSW_OK) return rc;
+  if (T == 0) return FSW_OK;
+  if (!x || !w || !ws || !y || !scratch) return fail(FSW_EINVAL, "NULL pointer");
+  if (!aligned16(x) || !aligned16(w) || !aligned16(y) || !aligned16(scratch))
+    return fail(FSW_EINVAL, "pointers must be 16-byte aligned");
+  if (scratch_bytes < fsw_fp8_linear_scratch_bytes(T, K)) return fail(FSW_EINVAL, "scratch of %lld bytes is too small", (long long)scratch_bytes);
+  DeviceInfo* dev = nullptr;
+  if ((rc = ensure_device(&dev)) != FSW_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* xq = static_cast<uint8_t*>(scratch);
+  float* xs = reinterpret_cast<float*>(xq + align256(T * K));
+  if ((rc = quantize_rows(x, xq, xs, T, T, K, dtype, nullptr, nullptr, st)) != FSW_OK) return rc;
+  const Fp8Rows r = {T, T, nullptr, nullptr};
+  return run_fp8(r, xq, xs, 1, T, w, static_cast<const float*>(ws), nullptr, nullptr, y, nullptr, nullptr, K, N, dtype, dev, st);
+}
+
+// Scratch: [plan] xq xs hq hs [ys], for T rows (dense) or the plan's.
+struct Fp8MlpBuffers {
+  int64_t xq, xs, hq, hs, ys, bytes;
+};
+static Fp8MlpBuffers fp8_mlp_buffers(int64_t plan_bytes, int64_t rows, int64_t d, int64_t f, int64_t ys_cols) {
+  Fp8MlpBuffers b;
+  b.xq = align256(plan_bytes);
+  b.xs = b.xq + align256(rows * d);
+  b.hq = b.xs + align256(rows * blocks_of(d) * 4);
+  b.hs = b.hq + align256(rows * f);
+  b.ys = b.hs + align256(rows * blocks_of(f) * 4);
+  b.bytes = b.ys + align256(rows * ys_cols * 2);
+  return b;
+}
+
+static int check_fp8_mlp(int64_t T, int64_t d, int64_t f, int64_t d_out, int dtype) {
+  int rc = check_fp8(T, d, f, dtype);
+  return rc != FSW_OK ? rc : check_fp8(T, f, d_out, dtype);
+}
+
+int64_t fsw_fp8_mlp_scratch_bytes(int64_t T, int64_t d, int64_t f) {
+  int rc = check_fp8_mlp(T, d, f, 8, FSW_BF16);
+  if (rc != FSW_OK) return rc;
+  return fp8_mlp_buffers(0, T, d, f, 0).bytes;
+}
+
+int fsw_fp8_mlp(const void* x, const void* w_gate, const void* s_gate, const void* w_up, const void* s_up,
+                const void* w_down, const void* s_down, void* y, void* scratch, int64_t scratch_bytes, int64_t T, int64_t d,
+                int64_t f, int64_t d_out, int dtype, void* stream) {
+  int rc = check_fp8_mlp(T, d, f, d_out, dtype);
+  if (rc != FSW_OK) return rc;
+  if (T == 0) return FSW_OK;
+  if (!x || !w_gate || !s_gate || !w_up || !s_up || !w_down || !s_down || !y || !scratch) return fail(FSW_EINVAL, "NULL pointer");
+  if (!aligned16(x) || !aligned16(w_gate) || !aligned16(w_up) || !aligned16(w_down) || !aligned16(y) || !aligned16(scratch))
+    return fail(FSW_EINVAL, "pointers must be 16-byte aligned");
+  const Fp8MlpBuffers b = fp8_mlp_buffers(0, T, d, f, 0);
+  if (scratch_bytes < b.bytes) return fail(FSW_EINVAL, "scratch of %lld bytes is too small", (long long)scratch_bytes);
+  DeviceInfo* dev = nullptr;
+  if ((rc = ensure_device(&dev)) != FSW_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* s = static_cast<char*>(scratch);
+  float *xs = reinterpret_cast<float*>(s + b.xs), *hs = reinterpret_cast<float*>(s + b.hs);
+  uint8_t* hq = reinterpret_cast<uint8_t*>(s + b.hq);
+  if ((rc = quantize_rows(x, s + b.xq, xs, T, T, d, dtype, nullptr, nullptr, st)) != FSW_OK) return rc;
+  const Fp8Rows r = {T, T, nullptr, nullptr};
+  if ((rc = run_fp8(r, s + b.xq, xs, 1, T, w_gate, static_cast<const float*>(s_gate), w_up, static_cast<const float*>(s_up),
+                    nullptr, hq, hs, d, f, dtype, dev, st)) != FSW_OK)
+    return rc;
+  return run_fp8(r, hq, hs, 1, T, w_down, static_cast<const float*>(s_down), nullptr, nullptr, y, nullptr, nullptr, f, d_out,
+                 dtype, dev, st);
+}
+
+static int check_fp8_experts(int64_t T, int k, int E, int64_t d, int64_t f, int64_t d_out, int dtype, int wtype, ExpertPlan* plan) {
+  int rc = check_experts(T, k, E, d, f, d_out, dtype, wtype);
+  if (rc == FSW_OK) rc = check_fp8_mlp(T, d, f, d_out, dtype);
+  if (rc != FSW_OK) return rc;
+  if (!make_plan(plan, T, k, E, choose_tile_rows(T * k, E))) return fail(FSW_EINVAL, "too many tokens");
+  return FSW_OK;
+}
+
+int64_t fsw_fp8_experts_scratch_bytes(int64_t T, int k, int E, int64_t d, int64_t f, int64_t d_out) {
+  ExpertPlan plan;
+  int rc = check_fp8_experts(T, k, E, d, f, d_out, FSW_BF16, FSW_FP32, &plan);
+  if (rc != FSW_OK) return rc;
+  return fp8_mlp_buffers(plan.ints * 4, plan.rows, d, f, d_out).bytes;
+}
+
+int fsw_fp8_experts_forward(const void* x, const void* weights, const void* indices, const void* w_gate,
+                            const void* s_gate, const void* w_up, const void* s_up, const void* w_down,
+                            const void* s_down, void* y, void* scratch, int64_t scratch_bytes, int64_t T, int k, int E,
+                            int64_t d, int64_t f, int64_t d_out, int dtype, int weights_dtype, void* stream) {
+  ExpertPlan plan;
+  int rc = check_fp8_experts(T, k, E, d, f, d_out, dtype, weights_dtype, &plan);
+  if (rc != FSW_OK) return rc;
+  if (T == 0) return FSW_OK;
+  if (!x || !weights || !indices || !w_gate || !s_gate || !w_up || !s_up || !w_down || !s_down || !y || !scratch)
+    return fail(FSW_EINVAL, "NULL pointer");
+  if (!aligned16(x) || !aligned16(w_gate) || !aligned16(w_up) || !aligned16(w_down) || !aligned16(y) || !aligned16(scratch))
+    return fail(FSW_EINVAL, "pointers must be 16-byte aligned");
+  const Fp8MlpBuffers b = fp8_mlp_buffers(plan.ints * 4, plan.rows, d, f, d_out);
+  if (scratch_bytes < b.bytes) return fail(FSW_EINVAL, "scratch of %lld bytes is too small", (long long)scratch_bytes);
+  DeviceInfo* dev = nullptr;
+  if ((rc = ensure_device(&dev)) != FSW_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* s = static_cast<char*>(scratch);
+  int* plan_dev = reinterpret_cast<int*>(s);
+  float *xs = reinterpret_cast<float*>(s + b.xs), *hs = reinterpret_cast<float*>(s + b.hs);
+  uint8_t* hq = reinterpret_cast<uint8_t*>(s + b.hq);
+  const int64_t R = plan.rows;
+  if ((rc = build_plan(plan, static_cast<const int*>(indices), plan_dev, st)) != FSW_OK) return rc;
+  if ((rc = quantize_rows(x, s + b.xq, xs, R, T, d, dtype, &plan, plan_dev, st)) != FSW_OK) return rc;
+  const Fp8Rows r = {R, plan.pairs, &plan, plan_dev};
+  if ((rc = run_fp8(r, s + b.xq, xs, 1, R, w_gate, static_cast<const float*>(s_gate), w_up, static_cast<const float*>(s_up),
+                    nullptr, hq, hs, d, f, dtype, dev, st)) != FSW_OK)
+    return rc;
+  if ((rc = run_fp8(r, hq, hs, 1, R, w_down, static_cast<const float*>(s_down), nullptr, nullptr, s + b.ys, nullptr, nullptr, f,
+                    d_out, dtype, dev, st)) != FSW_OK)
+    return rc;
+  return combine_rows(plan, plan_dev, s + b.ys, weights, weights_dtype, y, d_out, dtype, st);
+}
+
+}  // extern "C"

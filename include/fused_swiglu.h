@@ -315,6 +315,52 @@ int fsw_experts_backward(const void* dy, const void* weights, const void* w_gate
                          int k, int E, int64_t d, int64_t f, int64_t d_out, int dtype,
                          int weights_dtype, void* stream);
 
+/*
+ * Products in 8-bit floating point (e4m3) with a scale for each block of 128, for serving
+ * (no counterpart in the reference).  A quantised weight is (N, K) e4m3, K the inner size,
+ * with fp32 scales (ceil(N / 128), ceil(K / 128)), any positive numbers; a stack of E weights
+ * is dense.  Quantised rows are (T, K) e4m3 with one fp32 scale per row and 128 columns.
+ * K must be a multiple of 16, N of 8.
+ *
+ * fsw_fp8_quantize_rows: q (T, d), scales (ceil(d / 128), T) - block-major - of x (T, d) of
+ * `dtype`: the smallest power of two that brings the block's largest magnitude to 448 or
+ * less, 1 for a block of zeros, NaN for a block that holds inf or NaN.
+ * fsw_fp8_quantize_weight: w (E, d_in, d_out) -> q (E, d_out, d_in), scales
+ * (E, ceil(d_out / 128), ceil(d_in / 128)), the same rule.
+ * fsw_fp8_gemm: y (T, N) of `dtype` = rows @ weight^T; the rows' scale of block b of row t is
+ * xs[t * xs_row_stride + b * xs_block_stride].  fp32 accumulation.
+ * fsw_fp8_linear: quantises x (T, K) and multiplies.
+ * fsw_fp8_mlp: y = (silu(x Wg) * (x Wu)) Wd on quantised weights Wg, Wu (f, d), Wd (d_out, f);
+ * the gate's result is quantised like a row in the epilogue of the product that makes it.
+ * fsw_fp8_experts_forward: fsw_experts_forward on such weights, stacked (E, ...); d and f
+ * multiples of 16, d_out of 8.
+ * The *_scratch_bytes functions give the scratch a call needs (negative: bad sizes); calls
+ * that may overlap on the GPU need different scratch.
+ */
+int fsw_fp8_quantize_rows(const void* x, void* q, void* scales, int64_t T, int64_t d, int dtype,
+                          void* stream);
+int fsw_fp8_quantize_weight(const void* w, void* q, void* scales, int E, int64_t d_in,
+                            int64_t d_out, int dtype, void* stream);
+int fsw_fp8_gemm(const void* xq, const void* xs, int64_t xs_row_stride, int64_t xs_block_stride,
+                 const void* w, const void* ws, void* y, int64_t T, int64_t K, int64_t N,
+                 int dtype, void* stream);
+int64_t fsw_fp8_linear_scratch_bytes(int64_t T, int64_t K);
+int fsw_fp8_linear(const void* x, const void* w, const void* ws, void* y, void* scratch,
+                   int64_t scratch_bytes, int64_t T, int64_t K, int64_t N, int dtype,
+                   void* stream);
+int64_t fsw_fp8_mlp_scratch_bytes(int64_t T, int64_t d, int64_t f);
+int fsw_fp8_mlp(const void* x, const void* w_gate, const void* s_gate, const void* w_up,
+                const void* s_up, const void* w_down, const void* s_down, void* y, void* scratch,
+                int64_t scratch_bytes, int64_t T, int64_t d, int64_t f, int64_t d_out, int dtype,
+                void* stream);
+int64_t fsw_fp8_experts_scratch_bytes(int64_t T, int k, int E, int64_t d, int64_t f, int64_t d_out);
+int fsw_fp8_experts_forward(const void* x, const void* weights, const void* indices,
+                            const void* w_gate, const void* s_gate, const void* w_up,
+                            const void* s_up, const void* w_down, const void* s_down, void* y,
+                            void* scratch, int64_t scratch_bytes, int64_t T, int k, int E,
+                            int64_t d, int64_t f, int64_t d_out, int dtype, int weights_dtype,
+                            void* stream);
+
 /* Message for the last non-zero return on the calling thread ("" if none). */
 const char* fsw_last_error(void);
 

@@ -6,7 +6,8 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+# half a step of each type, relative: what one rounding is off by at most
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 
 
 def inputs(T, E, k, d, f, o, dtype, seed=0, spread=1.0, wdtype=None):
@@ -58,16 +59,15 @@ def run(x, w, idx, wg, wu, wd, dy=None):
 
 # Roundings between an input and each output: y passes g, u, h, its row and the sum
 # (5), dx dh, dg, du, its row and the sum on top of g and u (7), the weights' gradients at
-# most as many.  Each is at most a step (2^-8, 2^-11) of the value; they are independent, so
-# their root of squares bounds the norm of the error with room: sqrt(7) < 3, times half a step
-# each as the largest rounding.
+# most as many.  Each moves a value by HALF of it at most and, evenly spread over a step, by less
+# than half of that in the norm; they are independent: sqrt(7) * 0.5 HALF < 1.5 HALF.
 NAMES = ("y", "dx", "dweights", "dw_gate", "dw_up", "dw_down")
 
 
 def compare(got, want, dtype):
     for name, a, b in zip(NAMES, got, want):
         assert a.shape == b.shape
-        assert rel(a, b) <= 1.5 * STEP[dtype], (name, rel(a, b))
+        assert rel(a, b) <= 1.5 * HALF[dtype], (name, rel(a, b))
 
 
 SHAPES = [  # T, E, k, d, f, o
@@ -110,7 +110,7 @@ def test_gradient_against_differences():
         have = (grad.double() * v).sum().item()
         size = torch.linalg.norm(grad.double()).item() * torch.linalg.norm(v).item()
         # a norm-wise error of 1.5 steps in the gradient moves the product by at most that of |grad| |v|
-        assert abs(have - want) <= 1.5 * STEP[torch.float16] * size
+        assert abs(have - want) <= 1.5 * HALF[torch.float16] * size
 
 
 def test_experts_without_rows_dropped_pairs_and_repeated_indices():
@@ -229,8 +229,8 @@ def test_moe_block_router_and_experts_together(score):
             h = torch.nn.functional.silu(x64[t] @ wg[e]) * (x64[t] @ wu[e])
             out = out.index_add(0, t, w[t, j][:, None] * (h @ wd[e]))
     want = torch.autograd.grad(out, leaves, dy.view(74, 128).double())
-    assert rel(y.view(74, 128), out.detach()) < 2 * STEP[torch.bfloat16]
+    assert rel(y.view(74, 128), out.detach()) < 2 * HALF[torch.bfloat16]
     got = [x.grad.view(74, 128), m.w_router.grad, m.w_gate.grad, m.w_up.grad, m.w_down.grad]
     for name, a, b in zip(("x", "router", "gate", "up", "down"), got, want):
         # the logits' rounding (half a step of values up to 3) moves a weight by that much too
-        assert rel(a, b) < 3 * STEP[torch.bfloat16], (name, rel(a, b))
+        assert rel(a, b) < 3 * HALF[torch.bfloat16], (name, rel(a, b))
