@@ -342,9 +342,9 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
           __syncwarp();
           if (lane == 0) {
             if (CG == 2)
-              ptx::mbar_arrive_cluster(ptx::mapa(tempty_bar(a), 0));
+              ptx::mbar_arrive_cluster_relaxed(ptx::mapa(tempty_bar(a), 0));
             else
-              ptx::mbar_arrive(tempty_bar(a));
+              ptx::mbar_arrive_relaxed(tempty_bar(a));
           }
         };
         if (active) {
