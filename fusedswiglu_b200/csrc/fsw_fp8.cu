@@ -29,7 +29,7 @@ namespace fsw {
 namespace {
 
 constexpr int kBlock = 128;
-constexpr float kE4M3Max = 448.0f;
+constexpr int kMaxSplits = 8;  // portable cluster size
 
 struct Fp8Params {
   CUtensorMap a, b0, b1;
@@ -42,6 +42,7 @@ struct Fp8Params {
   int M, N;                 // output rows and columns
   int num_m_tiles, num_n_tiles, group_m;
   void* out;                // (M, N) of the output type
+  int wide_rows;            // every row of out starts on a 32-byte boundary
   uint8_t* hq;              // dual: (M, N) e4m3
   float* hs;                // dual: hs[block * hs_pitch + row]
   int64_t hs_pitch;
@@ -60,13 +61,22 @@ struct Fp8Cfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = CG == 2 ? 6 : 4;
   static constexpr int EPI_WARPS = 8;
-  static constexpr int EPI_BUF_BYTES = 32 * 128;
+  static constexpr int AMAX_BYTES = 2 * EPI_WARPS * 32 * 4;  // DUAL: row maxima, two tiles in turn
+  static constexpr int SCALE_SLOTS = 4;
+  static constexpr int SCALE_BYTES = SCALE_SLOTS * 2 * 128 * 4;
   static constexpr int BAR_BYTES = 512;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * EPI_BUF_BYTES + BAR_BYTES + 1024;
-  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + AMAX_BYTES + SCALE_BYTES + BAR_BYTES + 1024;
+  // Three warpgroups: producer, MMA issuer, scale warp and an idle one; twice four epilogue warps.  The
+  // block starts with 168 registers a thread (168 * 384 = 64512); the first group keeps 104 and
+  // the others take 200 (104 * 128 + 200 * 256 = 64512): 128 sums, two chunks of 16 in flight.
+  static constexpr int THREADS = 128 + 32 * EPI_WARPS;
+  static constexpr int REGS_FIRST = 104, REGS_EPILOGUE = 200;
+  static_assert(REGS_FIRST * 128 + REGS_EPILOGUE * 32 * EPI_WARPS <= 168 * THREADS, "registers");
   static_assert(SMEM_BYTES <= kSmemBudget, "shared memory");
-  // a split tile's sums overlay the operand stages: 8 warps x 128 columns x 32 lanes
-  static_assert(EPI_WARPS * 128 * 32 * 4 <= STAGES * STAGE_BYTES, "partial sums");
+  // A split tile's sums overlay the operand stages: 128 rows of 256 columns, padded so that
+  // the 16-byte writes of lanes with adjacent rows fall into different banks.
+  static constexpr int PART_LD = 260;
+  static_assert(128 * PART_LD * 4 <= STAGES * STAGE_BYTES, "partial sums");
 };
 
 template <int CG>
@@ -137,10 +147,32 @@ __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d
   return lo | (hi << 16);
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+// Not volatile: the loads of all shares may be in flight together (the barriers around them are).
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
+}
+
+// Columns [col, col + 32) of a row of N, rounded to T; whole sectors where the rows are aligned.
+template <typename T>
+__device__ __forceinline__ void store_row32(T* row, int col, int N, bool wide, const float* v) {
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+  if (wide) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (col + h * 16 < N)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + col + h * 16),
+                     "r"(w[8 * h]), "r"(w[8 * h + 1]), "r"(w[8 * h + 2]), "r"(w[8 * h + 3]), "r"(w[8 * h + 4]),
+                     "r"(w[8 * h + 5]), "r"(w[8 * h + 6]), "r"(w[8 * h + 7])
+                     : "memory");
+  } else {
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+      if (col + h * 8 < N) ptx::st_global_v4(row + col + h * 8, w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
+  }
 }
 
 struct Fp8Work {
@@ -156,9 +188,10 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
   const uint32_t raw_u32 = ptx::smem_u32(smem_raw);
   const uint32_t smem_base = (raw_u32 + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - raw_u32);
-  const uint32_t epi_base = smem_base + STAGES * C::STAGE_BYTES;
-  const uint32_t amax_off = STAGES * C::STAGE_BYTES;  // DUAL: in place of the store buffers
-  const uint32_t bar_base = epi_base + C::EPI_WARPS * C::EPI_BUF_BYTES;
+  const uint32_t amax_off = STAGES * C::STAGE_BYTES;
+  // [slot][which of the tile's two weight blocks][row]: the row's scale times the block's
+  float* scale_ring = reinterpret_cast<float*>(smem_gen + amax_off + C::AMAX_BYTES);
+  const uint32_t bar_base = smem_base + amax_off + C::AMAX_BYTES + C::SCALE_BYTES;
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
   auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
@@ -177,7 +210,7 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
       ptx::mbar_init(empty_bar(s), 1);
     }
     for (int a = 0; a < 2; ++a) {
-      ptx::mbar_init(tfull_bar(a), 1);
+      ptx::mbar_init(tfull_bar(a), 2);  // the MMAs' commit and the scale warp
       ptx::mbar_init(tempty_bar(a), C::EPI_WARPS * CG);
     }
     *abort_flag = 0u;
@@ -223,7 +256,9 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
     return true;
   };
 
-  if (warp == 0) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_FIRST));
+   if (warp == 0) {
     // ======================= TMA producer (one thread) =======================
     if (lane == 0 && !p.stall_producer) {
       int s = 0;
@@ -244,11 +279,10 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
           if (CG == 1 || rank == 0) ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
           const int k0 = kb * kBlock;
           if constexpr (CG == 2) {
+            // each CTA stages one half of the tile's weight rows
             ptx::tma_load_2d_pair(a_dst, &p.a, fb, k0, m0, pol);
-            if (DUAL)
-              ptx::tma_load_3d_pair(b_dst, rank ? &p.b1 : &p.b0, fb, k0, n0, w.expert, pol);
-            else
-              ptx::tma_load_3d_pair(b_dst, &p.b0, fb, k0, n0 + static_cast<int>(rank) * 128, w.expert, pol);
+            ptx::tma_load_3d_pair(b_dst, (DUAL && rank) ? &p.b1 : &p.b0, fb, k0,
+                                  DUAL ? n0 : n0 + static_cast<int>(rank) * 128, w.expert, pol);
           } else {
             ptx::tma_load_2d(a_dst, &p.a, fb, k0, m0, pol);
             ptx::tma_load_3d(b_dst, &p.b0, fb, k0, n0, w.expert, pol);
@@ -261,7 +295,7 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
         }
       }
     }
-  } else if (warp == 1) {
+   } else if (warp == 1) {
     // ================ MMA issuer (one thread of the pair leader) ================
     if ((CG == 1 || rank == 0) && lane == 0) {
       int s = 0, a = 0;
@@ -277,7 +311,8 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
       for (int idx = 0; ok && get_work(idx, w); ++idx) {
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = bounded_wait_thread(full_bar(s), ph, ctl, WAIT_MMA_FULL);
-          if (ok) ok = bounded_wait_thread(tempty_bar(a), aph ^ 1u, ctl, WAIT_MMA_TMEM_EMPTY);
+          if (!ok) break;
+          ok = bounded_wait_thread(tempty_bar(a), aph ^ 1u, ctl, WAIT_MMA_TMEM_EMPTY);
           if (!ok) break;
           ptx::tc_fence_after_sync();
           const uint32_t a_addr = smem_base + s * C::STAGE_BYTES, b_addr = a_addr + C::A_BYTES;
@@ -285,8 +320,8 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
           for (int k = 0; k < kBlock / 32; ++k)
             mma_f8_ss<CG>(tmem_base + a * 256, p.desc | (((a_addr + k * 32u) & 0x3FFFFu) >> 4),
                           p.desc | (((b_addr + k * 32u) & 0x3FFFFu) >> 4), p.idesc, k != 0 ? 1u : 0u);
-          commit(empty_bar(s));
           commit(tfull_bar(a));
+          commit(empty_bar(s));
           a ^= 1;
           if (a == 0) aph ^= 1u;
           if (++s == STAGES) {
@@ -296,79 +331,130 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
         }
       }
     }
+   } else if (warp == 2) {
+    // ================ scales of each block's rows, for the epilogue ================
+    // Slot kb % 4 is written once the MMAs of block kb - 2 are complete: they began after the
+    // epilogue had finished with block kb - 4.  Global loads run kAhead blocks ahead: a load
+    // asked for one block before its use cost more time than the block's MMAs.
+    constexpr int kAhead = 4;
+    int n = 0;  // blocks of all tiles so far
+    bool ok = true;
+    Fp8Work w;
+    for (int idx = 0; ok && get_work(idx, w); ++idx) {
+      const int row0 = w.m_tile * 128 * CG + (CG == 2 ? static_cast<int>(rank) * 128 : 0);
+      const float* x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = row0 + i * 32 + lane;
+        x[i] = p.xs + static_cast<int64_t>(row < p.M ? row : p.M - 1) * p.xs_row;
+      }
+      const int nb = DUAL ? w.n_tile : 2 * w.n_tile;
+      const int64_t wbase = (static_cast<int64_t>(w.expert) * p.ws_rows + nb) * p.num_kb;
+      const float* w0 = p.ws0 + wbase;
+      // the second block of a tile may lie behind the weight's last
+      const float* w1 = DUAL ? p.ws1 + wbase : (nb + 1 < p.ws_rows ? w0 + p.num_kb : w0);
+      float xv[kAhead][4], wv[kAhead][2];
+      auto fetch = [&](int kb, int i) {
+        kb = kb < kb1 ? kb : kb1 - 1;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) xv[i][r] = x[r][kb * p.xs_block];
+        wv[i][0] = w0[kb];
+        wv[i][1] = w1[kb];
+      };
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) fetch(kb0 + i, i);
+      for (int kbase = kb0; kbase < kb1 && ok; kbase += kAhead) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (kbase + i < kb1 && ok) {
+            // block n - 2 used the same region: its phase is the one before
+            if (n >= 2) ok = bounded_wait_warp(tfull_bar(n & 1), ((n >> 1) - 1) & 1, ctl, WAIT_EPI_TMEM_FULL);
+            if (ok) {
+              float* slot = scale_ring + (n & 3) * 256 + lane;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                slot[r * 32] = xv[i][r] * wv[i][0];
+                slot[128 + r * 32] = xv[i][r] * wv[i][1];
+              }
+              __syncwarp();
+              if (lane == 0) ptx::mbar_arrive(tfull_bar(n & 1));
+              ++n;
+              fetch(kbase + i + kAhead, i);
+            }
+          }
+        }
+      }
+    }
+   }
   } else {
     // ======================= epilogue: scale, add, write =======================
-    const int q = warp & 3, ew = warp - 2, half = ew >> 2;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_EPILOGUE));
+    const int q = warp & 3, ew = warp - 4, half = ew >> 2;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
-    // Columns of this warp within a region: one weight block of 128, or, with two weights, the
-    // same 64 columns of both, so that a thread holds gate and up of its columns.
-    const uint32_t col_lo = DUAL ? half * 64 : half * 128;
-    const uint32_t col_hi = DUAL ? 128 + half * 64 : half * 128 + 64;
-    const uint32_t buf = epi_base + ew * C::EPI_BUF_BYTES;
+    // This warp's columns: the same 64 of each half of a block's 256, so that a thread holds
+    // gate and up of its columns.
+    const uint32_t my_tempty = (CG == 2) ? ptx::mapa(tempty_bar(0), 0) : tempty_bar(0);
     int a = 0;
     uint32_t aph = 0;
     bool ok = true;
-    int parity = 0;
+    int parity = 0, slot = 0;
     Fp8Work w;
     for (int idx = 0; ok && get_work(idx, w); ++idx) {
       const int tile_row = (CG == 2 ? static_cast<int>(rank) * 128 : 0) + q * 32;  // of this warp, in the tile
       const int row0 = w.m_tile * 128 * CG + tile_row;
       const bool active = tile_row < w.rows;  // no valid row here: nothing is added up or stored
-      const int row = row0 + lane < p.M ? row0 + lane : p.M - 1;
-      const int nb = DUAL ? w.n_tile : 2 * w.n_tile + half;
-      const bool have_block = nb < p.ws_rows;
-      const int64_t wbase = (static_cast<int64_t>(w.expert) * p.ws_rows + (have_block ? nb : 0)) * p.num_kb;
-      const float* xs = p.xs + static_cast<int64_t>(row) * p.xs_row;
       float acc[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
-      float x_next = 0.0f, lo_next = 0.0f, hi_next = 0.0f;
-      auto fetch = [&](int kb) {
-        if (active && kb < kb1) {
-          x_next = xs[kb * p.xs_block];
-          lo_next = p.ws0[wbase + kb];
-          hi_next = DUAL ? p.ws1[wbase + kb] : lo_next;
+      auto wait_block = [&]() {
+        ok = bounded_wait_warp(tfull_bar(a), aph, ctl, WAIT_EPI_TMEM_FULL);
+        if (ok) ptx::tc_fence_after_sync();
+        return ok;
+      };
+      auto release = [&]() {
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 2)
+            ptx::mbar_arrive_cluster_relaxed(my_tempty + 8u * a);
+          else
+            ptx::mbar_arrive_relaxed(my_tempty + 8u * a);
         }
       };
-      fetch(kb0);
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const float s_lo = x_next * lo_next, s_hi = x_next * hi_next;
-        fetch(kb + 1);
-        ok = bounded_wait_warp(tfull_bar(a), aph, ctl, WAIT_EPI_TMEM_FULL);
-        if (!ok) break;
-        ptx::tc_fence_after_sync();
-        auto release = [&]() {
-          ptx::tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) {
-            if (CG == 2)
-              ptx::mbar_arrive_cluster_relaxed(ptx::mapa(tempty_bar(a), 0));
-            else
-              ptx::mbar_arrive_relaxed(tempty_bar(a));
-          }
-        };
-        if (active) {
-          // eight chunks of 16 columns, two loads in flight
-          const uint32_t t0 = lane_base + a * 256;
-          uint32_t r0[16], r1[16];
-          ptx::tmem_ld_32x16(t0 + col_lo, r0);
+      auto next_block = [&]() {
+        a ^= 1;
+        if (a == 0) aph ^= 1u;
+        slot = (slot + 1) & (C::SCALE_SLOTS - 1);
+      };
+      if (!active) {
+        for (int kb = kb0; kb < kb1 && ok; ++kb) {
+          if (wait_block()) release();
+          next_block();
+        }
+      } else if (wait_block()) {
+        // eight chunks of 16 columns; the next one is on its way while one is added
+        const uint32_t t0 = lane_base + half * 64;
+        uint32_t r0[16], r1[16];
+        for (int kb = kb0;;) {
+          const uint32_t t = t0 + a * 256;
+          ptx::tmem_ld_32x16(t, r0);
+          const float* sc = scale_ring + slot * 256 + q * 32 + lane;
+          const float s_lo = sc[0], s_hi = sc[128];
 #pragma unroll
           for (int c = 0; c < 8; c += 2) {
             tmem_wait16(r0);
-            ptx::tmem_ld_32x16(t0 + (c + 1 < 4 ? col_lo + (c + 1) * 16 : col_hi + (c - 3) * 16), r1);
+            ptx::tmem_ld_32x16(t + (c < 4 ? (c + 1) * 16 : 64 + (c + 1) * 16), r1);
             scaled_add16(acc + c * 16, r0, c < 4 ? s_lo : s_hi);
             tmem_wait16(r1);
-            if (c + 2 < 8)
-              ptx::tmem_ld_32x16(t0 + (c + 2 < 4 ? col_lo + (c + 2) * 16 : col_hi + (c - 2) * 16), r0);
+            if (c < 6)
+              ptx::tmem_ld_32x16(t + (c < 2 ? (c + 2) * 16 : 64 + (c + 2) * 16), r0);
             else
               release();
-            scaled_add16(acc + (c + 1) * 16, r1, c + 1 < 4 ? s_lo : s_hi);
+            scaled_add16(acc + (c + 1) * 16, r1, c < 4 ? s_lo : s_hi);
           }
-        } else {
-          release();
+          next_block();
+          if (++kb == kb1 || !wait_block()) break;
         }
-        a ^= 1;
-        if (a == 0) aph ^= 1u;
       }
       // The two warps of a lane quadrant meet once a tile (below).  One that gives up arrives
       // there without waiting, and none waits once the flag is up: no warp is left behind.
@@ -379,25 +465,23 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
       }
 
       if (!DUAL && p.splits > 1) {
-        // partial sums of this share, [warp][column][lane]; added up behind the cluster barrier.
-        // Every MMA and load of this CTA is complete: the stages are free.
-        if (active) {
-          float* part = reinterpret_cast<float*>(smem_gen) + ew * 128 * 32 + lane;
+        // Partial sums of this share, added up behind the cluster barrier.  Every MMA and load of
+        // this CTA is complete: the stages are free.
+        if (active && tile_row + lane < w.rows) {
+          const uint32_t mine = smem_base + ((tile_row + lane) * C::PART_LD + half * 64) * 4;
 #pragma unroll
-          for (int i = 0; i < 128; ++i) part[i * 32] = acc[i];
+          for (int i = 0; i < 32; ++i)
+            ptx::st_shared_v4(mine + ((i >> 4) * 128 + (i & 15) * 4) * 4, __float_as_uint(acc[4 * i]),
+                              __float_as_uint(acc[4 * i + 1]), __float_as_uint(acc[4 * i + 2]),
+                              __float_as_uint(acc[4 * i + 3]));
         }
       } else if constexpr (!DUAL) {
-        if (active) {
+        // a thread holds 64 consecutive columns of its row in each half: whole sectors
+        if (active && row0 + lane < p.M) {
+          T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(row0 + lane) * p.N;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t pk[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) pk[i] = pack2<T>(acc[j * 64 + 2 * i], acc[j * 64 + 2 * i + 1]);
-            stage_rows128(buf, lane, pk);
-            __syncwarp();
-            flush_rows128(buf, lane, p.out, row0, w.n_tile * 256 + half * 128 + j * 64, p.M, p.N, p.N);
-            __syncwarp();
-          }
+          for (int j = 0; j < 4; ++j)
+            store_row32<T>(dst, w.n_tile * 256 + (j >> 1) * 128 + half * 64 + (j & 1) * 32, p.N, p.wide_rows != 0, acc + j * 32);
         }
       } else {
         // h = silu(g) u in fp32; the row's block of 128 columns is shared by the two warps of
@@ -442,26 +526,30 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
     ptx::cluster_arrive();
     ptx::cluster_wait();
     Fp8Work w;
-    if (warp >= 2 && get_work(0, w)) {
-      const int q = warp & 3, ew = warp - 2, half = ew >> 2;
-      const int row = w.m_tile * 128 + q * 32 + lane;
-      if (q * 32 < w.rows) {
-        // this CTA adds and writes columns [rank * per, (rank + 1) * per) of each warp's 128
-        const int per = 128 / p.splits;
-        for (int c0 = static_cast<int>(rank) * per; c0 < (static_cast<int>(rank) + 1) * per; c0 += 8) {
-          float sum[8];
+    if (warp >= 4 && get_work(0, w) && *abort_flag == 0u) {
+      // This CTA adds and writes 4-column groups [g0, g1) of the tile's 64, shares in order.
+      const int g0 = 64 * static_cast<int>(rank) / p.splits, g1 = 64 * (static_cast<int>(rank) + 1) / p.splits;
+      const int rows = w.rows < 128 ? w.rows : 128, groups = g1 - g0;
+      for (int i = threadIdx.x - 128; i < rows * groups; i += 32 * C::EPI_WARPS) {
+        const int r = i / groups, g = g0 + i - r * groups;
+        const uint32_t at = smem_base + (r * C::PART_LD + g * 4) * 4;
+        float4 v[kMaxSplits];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
-          for (int r = 0; r < p.splits; ++r) {
-            const uint32_t base = ptx::mapa(smem_base + ((ew * 128 + c0) * 32 + lane) * 4u, r);
+        for (int c = 0; c < kMaxSplits; ++c)
+          if (c < p.splits) v[c] = ld_cluster_f32x4(ptx::mapa(at, c));
+        float4 sum = v[0];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] += ld_cluster_f32(base + i * 128u);
+        for (int c = 1; c < kMaxSplits; ++c)
+          if (c < p.splits) {
+            sum.x += v[c].x;
+            sum.y += v[c].y;
+            sum.z += v[c].z;
+            sum.w += v[c].w;
           }
-          const int col = w.n_tile * 256 + half * 128 + c0;
-          if (row < p.M && col < p.N && *abort_flag == 0u)
-            ptx::st_global_v4(static_cast<T*>(p.out) + static_cast<int64_t>(row) * p.N + col, pack2<T>(sum[0], sum[1]),
-                              pack2<T>(sum[2], sum[3]), pack2<T>(sum[4], sum[5]), pack2<T>(sum[6], sum[7]));
-        }
+        const int col = w.n_tile * 256 + g * 4;
+        if (col < p.N)
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + static_cast<int64_t>(w.m_tile * 128 + r) * p.N + col) =
+              make_uint2(pack2<T>(sum.x, sum.y), pack2<T>(sum.z, sum.w));
       }
     }
     __syncwarp();
@@ -598,6 +686,39 @@ int launch_fp8_one(const Fp8Params& p, int grid, cudaStream_t st) {
   return FSW_OK;
 }
 
+// How many clusters of c single-CTA tiles can be resident at once on the current device.
+int resident_clusters(int c, int* fit) {
+  static std::atomic<int> known[64][kMaxSplits + 1];  // value + 1; 0 = not asked yet
+  int dev = 0;
+  FSW_CUDA(cudaGetDevice(&dev));
+  std::atomic<int>& slot = known[dev & 63][c];
+  int v = slot.load();
+  if (v == 0) {
+    FSW_CUDA(cudaFuncSetAttribute(fp8_gemm_kernel<1, false, __nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  Fp8Cfg<1>::SMEM_BYTES));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c * 256, 1, 1);
+    cfg.blockDim = dim3(Fp8Cfg<1>::THREADS, 1, 1);
+    cfg.dynamicSmemBytes = Fp8Cfg<1>::SMEM_BYTES;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = c;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, fp8_gemm_kernel<1, false, __nv_bfloat16>, &cfg) != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+    v = n + 1;
+    slot.store(v);
+  }
+  *fit = v - 1;
+  return FSW_OK;
+}
+
 // The rows an 8-bit product works on: T dense rows, or a plan's.
 struct Fp8Rows {
   int64_t rows;                 // of the arrays
@@ -629,8 +750,19 @@ int run_fp8(const Fp8Rows& r, const void* xq, const float* xs, int64_t xs_row, i
   if (tiles >= (1ll << 30)) return fail(FSW_EINVAL, "too many tiles");
   p.splits = 1;
   if (cg == 1 && !dual && r.plan == nullptr) {
-    // fewer tiles than half the SMs: divide their K blocks, at least 4 blocks a share
-    while (p.splits < 8 && tiles * p.splits * 2 <= d->sm_count && p.num_kb >= 8 * p.splits) p.splits *= 2;
+    // Fewer tiles than SMs: divide their K blocks, at least 4 a share, over as many CTAs as
+    // leave all clusters resident at once (a GPC holds whole clusters only: of 8 CTAs 16 fit,
+    // not 148 / 8, and a 17th cluster would double the time).
+    for (int c = kMaxSplits; c > 1; --c) {
+      if (p.num_kb < 4 * c || tiles * c > d->sm_count) continue;
+      int fit = 0;
+      const int rc = resident_clusters(c, &fit);
+      if (rc != FSW_OK) return rc;
+      if (tiles <= fit) {
+        p.splits = c;
+        break;
+      }
+    }
   }
   p.a_rows = r.most > 120 ? 128 : (int)((r.most + 7) / 8 * 8);
   if (cg == 2) p.a_rows = 128;
@@ -651,6 +783,7 @@ int run_fp8(const Fp8Rows& r, const void* xq, const float* xs, int64_t xs_row, i
   p.M = (int)r.rows;
   p.N = (int)N;
   p.out = out;
+  p.wide_rows = (N & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 31u) == 0;
   p.hq = hq;
   p.hs = hs;
   p.hs_pitch = r.rows;
