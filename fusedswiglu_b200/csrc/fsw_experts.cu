@@ -122,6 +122,7 @@ template <bool whole>
 __global__ void __launch_bounds__(kPlanWarps * 32) plan_count_kernel(const ExpertPlan p, const int* indices, int* plan) {
   extern __shared__ int hist[];  // [kPlanWarps][E]
   __shared__ int warp_sums[kPlanWarps];
+  ptx::allow_successor();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int i = threadIdx.x; i < kPlanWarps * p.E; i += blockDim.x) hist[i] = 0;
   __syncthreads();
@@ -155,6 +156,8 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_count_kernel(const Exper
 // One block: block_hist[b][e] becomes the number of pairs of e before block b.
 __global__ void __launch_bounds__(1024) plan_place_kernel(const ExpertPlan p, int* plan) {
   __shared__ int warp_sums[32];
+  ptx::allow_successor();
+  ptx::wait_predecessor();
   place_experts(p, plan, warp_sums, [&](int e) {
     int c = 0;
     for (int b = 0; b < p.blocks; ++b) {
@@ -169,6 +172,8 @@ __global__ void __launch_bounds__(1024) plan_place_kernel(const ExpertPlan p, in
 
 __global__ void __launch_bounds__(kPlanWarps * 32) plan_rank_kernel(const ExpertPlan p, const int* indices, int* plan) {
   extern __shared__ int hist[];
+  ptx::allow_successor();
+  ptx::wait_predecessor();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int i = threadIdx.x; i < kPlanWarps * p.E; i += blockDim.x) hist[i] = 0;
   __syncthreads();
@@ -193,6 +198,8 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rank_kernel(const Expert
 // T + e clears the rows behind the last of expert e.
 __global__ void __launch_bounds__(128) gather_kernel(const ExpertPlan p, const int* __restrict__ plan,
                                                      const uint4* __restrict__ src, uint4* __restrict__ dst, int vecs) {
+  ptx::allow_successor();
+  ptx::wait_predecessor();
   if (blockIdx.x < static_cast<unsigned>(p.T)) {
     const int64_t t = blockIdx.x;
     const int* rows = plan + p.pair_row + t * p.k;
@@ -222,6 +229,8 @@ template <typename T, typename W, bool WEIGHTED>
 __global__ void __launch_bounds__(128) combine_kernel(const ExpertPlan p, const int* __restrict__ plan,
                                                       const uint4* __restrict__ src, const void* __restrict__ weights,
                                                       uint4* __restrict__ y, int vecs) {
+  ptx::allow_successor();
+  ptx::wait_predecessor();
   const int64_t t = blockIdx.x;
   const int* rows = plan + p.pair_row + t * p.k;
   for (int v = blockIdx.y * blockDim.x + threadIdx.x; v < vecs; v += blockDim.x * gridDim.y) {
@@ -272,6 +281,8 @@ __global__ void __launch_bounds__(256) expert_gate_kernel(const ExpertPlan p, co
                                                           const uint4* __restrict__ u, const void* __restrict__ weights,
                                                           uint4* __restrict__ du, uint4* __restrict__ hs,
                                                           void* dweights, int vecs) {
+  ptx::allow_successor();
+  ptx::wait_predecessor();
   const int64_t row = blockIdx.x;
   if (row >= plan[1]) return;
   const int pair = plan[p.row_pair + row];
@@ -330,6 +341,8 @@ __global__ void __launch_bounds__(256) expert_gate_kernel(const ExpertPlan p, co
 // A pair whose index is outside [0, E) has no row: its weight's gradient is zero.
 template <typename W>
 __global__ void __launch_bounds__(256) dropped_weights_kernel(const ExpertPlan p, const int* __restrict__ plan, W* dweights) {
+  ptx::allow_successor();
+  ptx::wait_predecessor();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i < p.pairs && plan[p.pair_row + i] < 0) dweights[i] = W(0.0f);
 }
@@ -338,67 +351,59 @@ __global__ void __launch_bounds__(256) dropped_weights_kernel(const ExpertPlan p
 
 int build_plan(const ExpertPlan& p, const int* indices, int* plan, cudaStream_t st) {
   const size_t smem = sizeof(int) * kPlanWarps * p.E;  // at most 32 KB
+  const int threads = kPlanWarps * 32;
   if (p.blocks <= 1) {
-    plan_count_kernel<true><<<1, kPlanWarps * 32, smem, st>>>(p, indices, plan);
-    ++g_kernel_launches;
-  } else {
-    plan_count_kernel<false><<<p.blocks, kPlanWarps * 32, smem, st>>>(p, indices, plan);
-    plan_place_kernel<<<1, 1024, 0, st>>>(p, plan);
-    plan_rank_kernel<<<p.blocks, kPlanWarps * 32, smem, st>>>(p, indices, plan);
-    g_kernel_launches += 3;
+    FSW_CUDA(launch_dependent(plan_count_kernel<true>, dim3(1), threads, smem, st, false, 1, p, indices, plan));
+    return FSW_OK;
   }
-  FSW_CUDA(cudaGetLastError());
+  FSW_CUDA(launch_dependent(plan_count_kernel<false>, dim3(p.blocks), threads, smem, st, false, 1, p, indices, plan));
+  FSW_CUDA(launch_dependent(plan_place_kernel, dim3(1), 1024, 0, st, true, 1, p, plan));
+  FSW_CUDA(launch_dependent(plan_rank_kernel, dim3(p.blocks), threads, smem, st, true, 1, p, indices, plan));
   return FSW_OK;
 }
 
 int gather_rows(const ExpertPlan& p, const int* plan, const void* src, void* dst, int64_t row_bytes,
-                bool zero_padding, cudaStream_t st) {
-  ++g_kernel_launches;
-  gather_kernel<<<p.T + (zero_padding ? p.E : 0), 128, 0, st>>>(p, plan, static_cast<const uint4*>(src),
-                                                                static_cast<uint4*>(dst), (int)(row_bytes / 16));
-  FSW_CUDA(cudaGetLastError());
+                bool zero_padding, bool dependent, cudaStream_t st) {
+  FSW_CUDA(launch_dependent(gather_kernel, dim3(p.T + (zero_padding ? p.E : 0)), 128, 0, st, dependent, 1, p, plan,
+                            static_cast<const uint4*>(src), static_cast<uint4*>(dst), (int)(row_bytes / 16)));
   return FSW_OK;
 }
 
 template <typename T>
-static void launch_combine(const ExpertPlan& p, const int* plan, const void* src, const void* weights, int wtype, void* y,
-                           int vecs, cudaStream_t st) {
+static cudaError_t launch_combine(const ExpertPlan& p, const int* plan, const void* src, const void* weights, int wtype,
+                                  void* y, int vecs, cudaStream_t st) {
   const uint4* s = static_cast<const uint4*>(src);
   uint4* o = static_cast<uint4*>(y);
   // a row per block; a row of few tokens is cut into pieces so that the GPU has some to do
   dim3 grid(p.T, p.T >= 512 ? 1 : (vecs + 127) / 128);
   if (weights == nullptr)
-    combine_kernel<T, float, false><<<grid, 128, 0, st>>>(p, plan, s, weights, o, vecs);
-  else if (wtype == FSW_FP32)
-    combine_kernel<T, float, true><<<grid, 128, 0, st>>>(p, plan, s, weights, o, vecs);
-  else
-    combine_kernel<T, T, true><<<grid, 128, 0, st>>>(p, plan, s, weights, o, vecs);
+    return launch_dependent(combine_kernel<T, float, false>, grid, 128, 0, st, true, 1, p, plan, s, weights, o, vecs);
+  if (wtype == FSW_FP32)
+    return launch_dependent(combine_kernel<T, float, true>, grid, 128, 0, st, true, 1, p, plan, s, weights, o, vecs);
+  return launch_dependent(combine_kernel<T, T, true>, grid, 128, 0, st, true, 1, p, plan, s, weights, o, vecs);
 }
 
 int combine_rows(const ExpertPlan& p, const int* plan, const void* src, const void* weights, int wtype, void* y,
                  int64_t cols, int dtype, cudaStream_t st) {
-  ++g_kernel_launches;
   if (dtype == FSW_BF16)
-    launch_combine<__nv_bfloat16>(p, plan, src, weights, wtype, y, (int)(cols / 8), st);
+    FSW_CUDA(launch_combine<__nv_bfloat16>(p, plan, src, weights, wtype, y, (int)(cols / 8), st));
   else
-    launch_combine<__half>(p, plan, src, weights, wtype, y, (int)(cols / 8), st);
-  FSW_CUDA(cudaGetLastError());
+    FSW_CUDA(launch_combine<__half>(p, plan, src, weights, wtype, y, (int)(cols / 8), st));
   return FSW_OK;
 }
 
 template <typename T, typename W>
-static void launch_gate(const ExpertPlan& p, const int* plan, void* dh, const void* g, const void* u, const void* weights,
-                        void* du, void* hs, void* dweights, int64_t cols, cudaStream_t st) {
+static int launch_gate(const ExpertPlan& p, const int* plan, void* dh, const void* g, const void* u, const void* weights,
+                       void* du, void* hs, void* dweights, int64_t cols, cudaStream_t st) {
   const int vecs = (int)(cols / 8);
   const int threads = vecs >= 256 ? 256 : vecs > 64 ? 128 : 64;
-  expert_gate_kernel<T, W><<<p.rows, threads, 0, st>>>(p, plan, static_cast<uint4*>(dh), static_cast<const uint4*>(g),
-                                                      static_cast<const uint4*>(u), weights, static_cast<uint4*>(du),
-                                                      static_cast<uint4*>(hs), dweights, vecs);
-  ++g_kernel_launches;
-  if (dweights != nullptr) {
-    dropped_weights_kernel<W><<<(p.pairs + 255) / 256, 256, 0, st>>>(p, plan, static_cast<W*>(dweights));
-    ++g_kernel_launches;
-  }
+  FSW_CUDA(launch_dependent(expert_gate_kernel<T, W>, dim3(p.rows), threads, 0, st, true, 1, p, plan,
+                            static_cast<uint4*>(dh), static_cast<const uint4*>(g), static_cast<const uint4*>(u), weights,
+                            static_cast<uint4*>(du), static_cast<uint4*>(hs), dweights, vecs));
+  if (dweights != nullptr)
+    FSW_CUDA(launch_dependent(dropped_weights_kernel<W>, dim3((p.pairs + 255) / 256), 256, 0, st, true, 1, p, plan,
+                              static_cast<W*>(dweights)));
+  return FSW_OK;
 }
 
 // -------------------------------------------------------------------- GEMMs --
@@ -415,20 +420,8 @@ int launch_grouped_one(const GemmParams& p, int grid, cudaStream_t st) {
                                   TileCfg<MODE, CG, NSUB>::SMEM_BYTES));
     prepared.fetch_or(1ull << (dev & 63));
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(TileCfg<MODE, CG, NSUB>::THREADS, 1, 1);
-  cfg.dynamicSmemBytes = TileCfg<MODE, CG, NSUB>::SMEM_BYTES;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  ++g_kernel_launches;
-  FSW_CUDA(cudaLaunchKernelEx(&cfg, gemm_kernel<MODE, CG, NSUB, T, false>, p));
+  FSW_CUDA(launch_dependent(gemm_kernel<MODE, CG, NSUB, T, false>, dim3(grid), TileCfg<MODE, CG, NSUB>::THREADS,
+                            TileCfg<MODE, CG, NSUB>::SMEM_BYTES, st, true, CG, p));
   return FSW_OK;
 }
 
@@ -679,7 +672,7 @@ int fsw_experts_forward(const void* x, const void* weights, const void* indices,
   int* plan = reinterpret_cast<int*>(keep);
   x_.plan_dev = plan;
   if ((rc = build_plan(x_.plan, static_cast<const int*>(indices), plan, x_.st)) != FSW_OK) return rc;
-  if ((rc = gather_rows(x_.plan, plan, x, keep + b.xs, d * 2, train, x_.st)) != FSW_OK) return rc;
+  if ((rc = gather_rows(x_.plan, plan, x, keep + b.xs, d * 2, train, true, x_.st)) != FSW_OK) return rc;
   if ((rc = x_.swiglu(keep + b.xs, w_gate, w_up, tmp + b.h, train ? keep + b.g : nullptr, train ? keep + b.u : nullptr)) != FSW_OK)
     return rc;
   if ((rc = x_.product<MODE_GNN>(tmp + b.h, w_down, tmp + b.ys, f, d_out, false)) != FSW_OK) return rc;
@@ -723,21 +716,13 @@ int fsw_experts_backward(const void* dy, const void* weights, const void* w_gate
   char* tmp = static_cast<char*>(scratch);
   const int* plan = reinterpret_cast<const int*>(keep);
   x_.plan_dev = plan;
-  if ((rc = gather_rows(x_.plan, plan, dy, tmp + b.dys, d_out * 2, true, st)) != FSW_OK) return rc;
+  if ((rc = gather_rows(x_.plan, plan, dy, tmp + b.dys, d_out * 2, true, false, st)) != FSW_OK) return rc;
   if ((rc = x_.product<MODE_GNT>(tmp + b.dys, w_down, tmp + b.dh, d_out, f, true)) != FSW_OK) return rc;
   void* hs = dw_down ? tmp + b.hs : nullptr;
-  if (dtype == FSW_BF16) {
-    if (weights_dtype == FSW_FP32)
-      launch_gate<__nv_bfloat16, float>(x_.plan, plan, tmp + b.dh, keep + b.g, keep + b.u, weights, tmp + b.du, hs, dweights, f, st);
-    else
-      launch_gate<__nv_bfloat16, __nv_bfloat16>(x_.plan, plan, tmp + b.dh, keep + b.g, keep + b.u, weights, tmp + b.du, hs, dweights, f, st);
-  } else {
-    if (weights_dtype == FSW_FP32)
-      launch_gate<__half, float>(x_.plan, plan, tmp + b.dh, keep + b.g, keep + b.u, weights, tmp + b.du, hs, dweights, f, st);
-    else
-      launch_gate<__half, __half>(x_.plan, plan, tmp + b.dh, keep + b.g, keep + b.u, weights, tmp + b.du, hs, dweights, f, st);
-  }
-  FSW_CUDA(cudaGetLastError());
+  const bool w32 = weights_dtype == FSW_FP32;
+  auto* gate = dtype == FSW_BF16 ? (w32 ? launch_gate<__nv_bfloat16, float> : launch_gate<__nv_bfloat16, __nv_bfloat16>)
+                                 : (w32 ? launch_gate<__half, float> : launch_gate<__half, __half>);
+  if ((rc = gate(x_.plan, plan, tmp + b.dh, keep + b.g, keep + b.u, weights, tmp + b.du, hs, dweights, f, st)) != FSW_OK) return rc;
   const char *dg = tmp + b.dh, *du = tmp + b.du;  // dg took dh's place
   if (dw_down && (rc = x_.grad_weight<MODE_GTN>(hs, tmp + b.dys, nullptr, dw_down, nullptr, f, d_out)) != FSW_OK) return rc;
   if (dx) {

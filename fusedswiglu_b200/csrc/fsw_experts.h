@@ -60,7 +60,7 @@ int build_plan(const ExpertPlan& p, const int* indices, int* plan, cudaStream_t 
 
 // dst[row] = src[token of row] for 16-byte multiples of `row_bytes`; optionally zeros the padding.
 int gather_rows(const ExpertPlan& p, const int* plan, const void* src, void* dst, int64_t row_bytes,
-                bool zero_padding, cudaStream_t st);
+                bool zero_padding, bool dependent, cudaStream_t st);
 
 // y[t] = sum over j of weight[t, j] * src[row of (t, j)], in fp32, rounded once.
 // weights: nullptr for 1, else of type wtype (FSW_FP32 or dtype).

@@ -234,6 +234,12 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
   ptx::tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
 
+  ptx::allow_successor();
+  // The kernel ahead makes the rows (and the plan); a dense weight is older than both, so the
+  // producer fills the pipeline with its tiles before it waits.
+  const bool early = p.grp_meta == nullptr && warp == 0 && lane == 0 && !p.stall_producer;
+  if (!early) ptx::wait_predecessor();
+
   const int cluster = CG * p.splits;
   const int num_clusters = gridDim.x / cluster, cluster_id = blockIdx.x / cluster;
   const int m_tiles = p.grp_meta != nullptr ? p.grp_meta[0] : p.num_m_tiles;
@@ -267,27 +273,46 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
       const uint64_t pol = ptx::make_l2_policy(2);
       const uint32_t bytes = CG * (static_cast<uint32_t>(p.a_rows) * kBlock + C::B_BYTES);
       Fp8Work w;
+      auto row_of = [&]() { return w.m_tile * 128 * CG + (CG == 2 ? static_cast<int>(rank) * 128 : 0); };
+      auto bar_of = [&](int st) { return CG == 2 ? ptx::mapa(full_bar(st), 0) : full_bar(st); };
+      auto load_rows = [&](int kb, int st) {
+        const uint32_t dst = smem_base + st * C::STAGE_BYTES;
+        if constexpr (CG == 2)
+          ptx::tma_load_2d_pair(dst, &p.a, bar_of(st), kb * kBlock, row_of(), pol);
+        else
+          ptx::tma_load_2d(dst, &p.a, full_bar(st), kb * kBlock, row_of(), pol);
+      };
+      auto load_weight = [&](int kb, int st) {
+        const uint32_t dst = smem_base + st * C::STAGE_BYTES + C::A_BYTES;
+        const int k0 = kb * kBlock, n0 = w.n_tile * (DUAL ? 128 : 256);
+        if (CG == 1 || rank == 0) ptx::mbar_arrive_expect_tx(full_bar(st), bytes);
+        if constexpr (CG == 2) {
+          // each CTA stages one half of the tile's weight rows
+          ptx::tma_load_3d_pair(dst, (DUAL && rank) ? &p.b1 : &p.b0, bar_of(st), k0,
+                                DUAL ? n0 : n0 + static_cast<int>(rank) * 128, w.expert, pol);
+        } else {
+          ptx::tma_load_3d(dst, &p.b0, full_bar(st), k0, n0, w.expert, pol);
+          ptx::tma_load_3d(dst + 128 * kBlock, DUAL ? &p.b1 : &p.b0, full_bar(st), k0, DUAL ? n0 : n0 + 128, w.expert, pol);
+        }
+      };
+      int ahead = 0;  // blocks of the first tile whose weight tiles are on their way
+      if (early) {
+        if (get_work(0, w)) {
+          ahead = kb1 - kb0 < STAGES ? kb1 - kb0 : STAGES;
+          for (int i = 0; i < ahead; ++i) load_weight(kb0 + i, i);
+        }
+        ptx::wait_predecessor();
+      }
       for (int idx = 0; ok && get_work(idx, w); ++idx) {
-        const int m0 = w.m_tile * 128 * CG + (CG == 2 ? rank * 128 : 0);
-        const int n0 = w.n_tile * (DUAL ? 128 : 256);
         for (int kb = kb0; kb < kb1; ++kb) {
-          ok = bounded_wait_thread(empty_bar(s), ph ^ 1u, ctl, WAIT_PRODUCER_EMPTY);
-          if (!ok) break;
-          const uint32_t a_dst = smem_base + s * C::STAGE_BYTES, b_dst = a_dst + C::A_BYTES;
-          uint32_t fb = full_bar(s);
-          if (CG == 2) fb = ptx::mapa(fb, 0);
-          if (CG == 1 || rank == 0) ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
-          const int k0 = kb * kBlock;
-          if constexpr (CG == 2) {
-            // each CTA stages one half of the tile's weight rows
-            ptx::tma_load_2d_pair(a_dst, &p.a, fb, k0, m0, pol);
-            ptx::tma_load_3d_pair(b_dst, (DUAL && rank) ? &p.b1 : &p.b0, fb, k0,
-                                  DUAL ? n0 : n0 + static_cast<int>(rank) * 128, w.expert, pol);
+          if (ahead > 0) {
+            --ahead;  // the pipeline is empty: stage s is kb - kb0
           } else {
-            ptx::tma_load_2d(a_dst, &p.a, fb, k0, m0, pol);
-            ptx::tma_load_3d(b_dst, &p.b0, fb, k0, n0, w.expert, pol);
-            ptx::tma_load_3d(b_dst + 128 * kBlock, DUAL ? &p.b1 : &p.b0, fb, k0, DUAL ? n0 : n0 + 128, w.expert, pol);
+            ok = bounded_wait_thread(empty_bar(s), ph ^ 1u, ctl, WAIT_PRODUCER_EMPTY);
+            if (!ok) break;
+            load_weight(kb, s);
           }
+          load_rows(kb, s);
           if (++s == STAGES) {
             s = 0;
             ph ^= 1u;
@@ -585,6 +610,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                             float* __restrict__ scales, int64_t pitch, int d,
                                                             const ExpertPlan plan, const int* __restrict__ plan_dev) {
+  ptx::allow_successor();
+  ptx::wait_predecessor();
   const int64_t t = blockIdx.x;
   const int k = plan_dev != nullptr ? plan.k : 1;
   for (int c0 = (blockIdx.y * 256 + threadIdx.x) * 8; c0 - static_cast<int>(threadIdx.x & 15) * 8 < d; c0 += gridDim.y * 256 * 8) {
@@ -660,7 +687,7 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const T* __restric
 
 // ------------------------------------------------------------------ launches --
 template <int CG, bool DUAL, typename T>
-int launch_fp8_one(const Fp8Params& p, int grid, cudaStream_t st) {
+int launch_fp8_one(const Fp8Params& p, int grid, bool dependent, cudaStream_t st) {
   static std::atomic<uint64_t> prepared{0};
   int dev = 0;
   FSW_CUDA(cudaGetDevice(&dev));
@@ -669,20 +696,8 @@ int launch_fp8_one(const Fp8Params& p, int grid, cudaStream_t st) {
                                   Fp8Cfg<CG>::SMEM_BYTES));
     prepared.fetch_or(1ull << (dev & 63));
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(Fp8Cfg<CG>::THREADS, 1, 1);
-  cfg.dynamicSmemBytes = Fp8Cfg<CG>::SMEM_BYTES;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG * p.splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  ++g_kernel_launches;
-  FSW_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<CG, DUAL, T>, p));
+  FSW_CUDA(launch_dependent(fp8_gemm_kernel<CG, DUAL, T>, dim3(grid), Fp8Cfg<CG>::THREADS, Fp8Cfg<CG>::SMEM_BYTES, st,
+                            dependent, CG * p.splits, p));
   return FSW_OK;
 }
 
@@ -730,7 +745,7 @@ struct Fp8Rows {
 // out (rows, N) = x @ w^T, or with w1 hq, hs = quantised silu(x w^T) * (x w1^T).
 int run_fp8(const Fp8Rows& r, const void* xq, const float* xs, int64_t xs_row, int64_t xs_block, const void* w,
             const float* ws, const void* w1, const float* ws1, void* out, uint8_t* hq, float* hs, int64_t K, int64_t N,
-            int dtype, DeviceInfo* d, cudaStream_t st) {
+            int dtype, DeviceInfo* d, cudaStream_t st, bool dependent = true) {
   const bool dual = w1 != nullptr;
   const int E = r.plan != nullptr ? r.plan->E : 1;
   const int tile_n = dual ? 128 : 256;
@@ -801,11 +816,11 @@ int run_fp8(const Fp8Rows& r, const void* xq, const float* xs, int64_t xs_row, i
   const int grid = (int)(p.splits > 1 ? tiles * p.splits : (tiles < workers ? tiles : workers) * cg);
   const bool bf = dtype == FSW_BF16;
   if (cg == 2) {
-    if (dual) return launch_fp8_one<2, true, __nv_bfloat16>(p, grid, st);
-    return bf ? launch_fp8_one<2, false, __nv_bfloat16>(p, grid, st) : launch_fp8_one<2, false, __half>(p, grid, st);
+    if (dual) return launch_fp8_one<2, true, __nv_bfloat16>(p, grid, dependent, st);
+    return bf ? launch_fp8_one<2, false, __nv_bfloat16>(p, grid, dependent, st) : launch_fp8_one<2, false, __half>(p, grid, dependent, st);
   }
-  if (dual) return launch_fp8_one<1, true, __nv_bfloat16>(p, grid, st);
-  return bf ? launch_fp8_one<1, false, __nv_bfloat16>(p, grid, st) : launch_fp8_one<1, false, __half>(p, grid, st);
+  if (dual) return launch_fp8_one<1, true, __nv_bfloat16>(p, grid, dependent, st);
+  return bf ? launch_fp8_one<1, false, __nv_bfloat16>(p, grid, dependent, st) : launch_fp8_one<1, false, __half>(p, grid, dependent, st);
 }
 
 int quantize_rows(const void* x, void* q, float* scales, int64_t pitch, int64_t T, int64_t d, int dtype,
@@ -813,14 +828,14 @@ int quantize_rows(const void* x, void* q, float* scales, int64_t pitch, int64_t 
   ExpertPlan none = {};
   // a block covers 2048 columns; few tokens are spread over more blocks
   const dim3 grid((unsigned)T, (unsigned)(T >= 1024 ? 1 : (d + 2047) / 2048));
-  ++g_kernel_launches;
+  const ExpertPlan pl = plan ? *plan : none;
   if (dtype == FSW_BF16)
-    quantize_rows_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(x), static_cast<uint8_t*>(q),
-                                                              scales, pitch, (int)d, plan ? *plan : none, plan_dev);
+    FSW_CUDA(launch_dependent(quantize_rows_kernel<__nv_bfloat16>, grid, 256, 0, st, plan != nullptr, 1,
+                              static_cast<const __nv_bfloat16*>(x), static_cast<uint8_t*>(q), scales, pitch, (int)d, pl,
+                              plan_dev));
   else
-    quantize_rows_kernel<__half><<<grid, 256, 0, st>>>(static_cast<const __half*>(x), static_cast<uint8_t*>(q), scales,
-                                                       pitch, (int)d, plan ? *plan : none, plan_dev);
-  FSW_CUDA(cudaGetLastError());
+    FSW_CUDA(launch_dependent(quantize_rows_kernel<__half>, grid, 256, 0, st, plan != nullptr, 1,
+                              static_cast<const __half*>(x), static_cast<uint8_t*>(q), scales, pitch, (int)d, pl, plan_dev));
   return FSW_OK;
 }
 
@@ -888,7 +903,7 @@ int fsw_fp8_gemm(const void* xq, const void* xs, int64_t xs_row_stride, int64_t 
   if ((rc = ensure_device(&dev)) != FSW_OK) return rc;
   const Fp8Rows r = {T, T, nullptr, nullptr};
   return run_fp8(r, xq, static_cast<const float*>(xs), xs_row_stride, xs_block_stride, w, static_cast<const float*>(ws),
-                 nullptr, nullptr, y, nullptr, nullptr, K, N, dtype, dev, static_cast<cudaStream_t>(stream));
+                 nullptr, nullptr, y, nullptr, nullptr, K, N, dtype, dev, static_cast<cudaStream_t>(stream), false);
 }
 
 int64_t fsw_fp8_linear_scratch_bytes(int64_t T, int64_t K) {

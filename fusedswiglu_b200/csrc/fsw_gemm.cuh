@@ -977,6 +977,10 @@ __global__ void __launch_bounds__(64 + 32 * FSW_EPI_WARPS, 1)
   const int cluster_id = blockIdx.x / CG;
   const int num_tiles = p.num_m_tiles * p.num_n_tiles;
   const int num_kb = p.num_k_blocks;
+  if (is_grouped(MODE)) {  // launched as dependent kernels of a call
+    ptx::allow_successor();
+    ptx::wait_predecessor();
+  }
   // The idx-th work item of this pair; the roles of both CTAs walk the same sequence.
   const int grp_m_tiles = (is_grouped(MODE) && !is_grouped_k(MODE)) ? p.grp_meta[0] : p.num_m_tiles;
   auto get_work = [&](int idx, WorkItem& w) {

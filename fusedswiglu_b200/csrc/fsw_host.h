@@ -62,6 +62,38 @@ int64_t opt_l2_out();
 int64_t opt_wait_limit_ms();
 int64_t opt_stall_producer();
 
+// Launches `kernel`.  With `dependent` it may be scheduled before the kernel ahead of it in the
+// stream has finished (and, if that one is, ahead of that one's results): it has to call
+// ptx::wait_predecessor before it touches anything another kernel of the chain writes or reads.
+// The first kernel of a call is launched without it, so a call starts after all earlier work.
+template <class... Params, class... Args>
+inline cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int block, size_t smem, cudaStream_t st,
+                                    bool dependent, int cluster, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (dependent) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  ++g_kernel_launches;
+  return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace fsw

@@ -50,6 +50,14 @@ __device__ __forceinline__ uint32_t mapa(uint32_t smem_addr, uint32_t rank) {
   return r;
 }
 
+// ------------------------------------------------- dependent launches in a stream --
+// A kernel launched with launch_dependent (fsw_host.h) may start while its predecessor runs;
+// wait_predecessor returns when the predecessor is complete and its results are visible.
+// At least one thread of every CTA of such a kernel calls it, so a chain completes in order.
+__device__ __forceinline__ void wait_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// The successor may be scheduled once all CTAs have said so (or have ended).
+__device__ __forceinline__ void allow_successor() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---------------------------------------------------------------- mbarrier --
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
