@@ -296,6 +296,21 @@ def wait_flags(flags_ptr: int, n: int, seq: int, like: torch.Tensor) -> None:
     _lib.check("fsw_wait_flags", rc)
 
 
+def _call(name: str, like: torch.Tensor, *args) -> None:
+    """One C call on ``like``'s device and its current stream.  The switch of the current
+    device, which costs as much as a small kernel's launch, is made only where it is one."""
+    fn = getattr(_lib.load(), name)
+    index = like.device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc != _lib.FSW_OK:
+        _lib.check(name, rc)
+
+
 _ROUTE_DTYPE_CODE = {**_DTYPE_CODE, torch.float32: _lib.FSW_FP32}
 _SCORE_CODE = {"softmax": _lib.FSW_SCORE_SOFTMAX, "sigmoid": _lib.FSW_SCORE_SIGMOID}
 
@@ -318,12 +333,10 @@ def route(logits: torch.Tensor, bias: Optional[torch.Tensor], top_k: int, score:
         bias = bias.detach().to(torch.float32).contiguous()
     weights = torch.empty((T, max(top_k, 0)), device=logits.device, dtype=torch.float32)
     indices = torch.empty((T, max(top_k, 0)), device=logits.device, dtype=torch.int32)
-    with torch.cuda.device(logits.device):
-        rc = _lib.load().fsw_route(
-            logits.data_ptr(), logits.stride(0) if T > 1 else E, bias.data_ptr() if bias is not None else None,
-            weights.data_ptr(), indices.data_ptr(), T, E, top_k, code, _SCORE_CODE[score], int(renormalize), scale,
-            num_groups, topk_groups, _stream(logits))
-    _lib.check("fsw_route", rc)
+    _call("fsw_route", logits,
+          logits.data_ptr(), logits.stride(0) if T > 1 else E, bias.data_ptr() if bias is not None else None,
+          weights.data_ptr(), indices.data_ptr(), T, E, top_k, code, _SCORE_CODE[score], int(renormalize), scale,
+          num_groups, topk_groups)
     return weights, indices
 
 
@@ -333,18 +346,15 @@ def route_backward(logits: torch.Tensor, indices: torch.Tensor, dweights: torch.
     _require_cuda(logits, indices, dweights)
     T, E = logits.shape
     dlogits = torch.empty((T, E), device=logits.device, dtype=logits.dtype)
-    with torch.cuda.device(logits.device):
-        rc = _lib.load().fsw_route_backward(
-            logits.data_ptr(), logits.stride(0) if T > 1 else E, indices.data_ptr(), dweights.data_ptr(),
-            dlogits.data_ptr(), T, E, indices.shape[1], _route_code(logits), _SCORE_CODE[score], int(renormalize),
-            scale, _stream(logits))
-    _lib.check("fsw_route_backward", rc)
+    _call("fsw_route_backward", logits,
+          logits.data_ptr(), logits.stride(0) if T > 1 else E, indices.data_ptr(), dweights.data_ptr(),
+          dlogits.data_ptr(), T, E, indices.shape[1], _route_code(logits), _SCORE_CODE[score], int(renormalize), scale)
     return dlogits
 
 
 def expert_indices(indices: torch.Tensor, num_experts: int) -> torch.Tensor:
     """(T, k) int32, contiguous; wider indices are clamped first so that none wraps into range."""
-    idx = indices.reshape(-1, indices.shape[-1])
+    idx = indices if indices.ndim == 2 else indices.reshape(-1, indices.shape[-1])
     if idx.dtype != torch.int32:
         idx = idx.clamp(-1, num_experts).to(torch.int32)
     return idx.contiguous()
@@ -379,12 +389,10 @@ def experts_forward(x: torch.Tensor, weights: torch.Tensor, indices: torch.Tenso
     saved = _scratch(saved_bytes, x) if save else None
     nbytes = forward_bytes if save else inference_bytes
     scratch = _scratch(nbytes, x)
-    with torch.cuda.device(x.device):
-        rc = _lib.load().fsw_experts_forward(
-            x.data_ptr(), weights.data_ptr(), indices.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
-            w_down.data_ptr(), y.data_ptr(), saved.data_ptr() if save else None, saved_bytes if save else 0,
-            scratch.data_ptr(), nbytes, T, k, E, d, f, d_out, code, _weights_code(weights, x), _stream(x))
-    _lib.check("fsw_experts_forward", rc)
+    _call("fsw_experts_forward", x,
+          x.data_ptr(), weights.data_ptr(), indices.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
+          y.data_ptr(), saved.data_ptr() if save else None, saved_bytes if save else 0, scratch.data_ptr(), nbytes, T,
+          k, E, d, f, d_out, code, _weights_code(weights, x))
     return y, saved
 
 
@@ -405,12 +413,10 @@ def experts_backward(dy: torch.Tensor, weights: torch.Tensor, w_gate: torch.Tens
     dwg, dwu = (torch.empty_like(w_gate), torch.empty_like(w_up)) if need_gate_up else (None, None)
     dwd = torch.empty_like(w_down) if need_down else None
     ptr = lambda t: t.data_ptr() if t is not None else None
-    with torch.cuda.device(dy.device):
-        rc = _lib.load().fsw_experts_backward(
-            dy.data_ptr(), weights.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
-            saved.data_ptr(), saved_bytes, scratch.data_ptr(), backward_bytes, ptr(dx), ptr(dr), ptr(dwg), ptr(dwu),
-            ptr(dwd), T, k, E, d, f, d_out, _code(dy), _weights_code(weights, dy), _stream(dy))
-    _lib.check("fsw_experts_backward", rc)
+    _call("fsw_experts_backward", dy,
+          dy.data_ptr(), weights.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), saved.data_ptr(),
+          saved_bytes, scratch.data_ptr(), backward_bytes, ptr(dx), ptr(dr), ptr(dwg), ptr(dwu), ptr(dwd), T, k, E, d,
+          f, d_out, _code(dy), _weights_code(weights, dy))
     return dx, dr, dwg, dwu, dwd
 
 
@@ -433,9 +439,7 @@ def fp8_quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     T, d = x.shape
     q = torch.empty((T, d), device=x.device, dtype=torch.float8_e4m3fn)
     scale = torch.empty((_blocks(d), T), device=x.device, dtype=torch.float32)
-    with torch.cuda.device(x.device):
-        rc = _lib.load().fsw_fp8_quantize_rows(x.data_ptr(), q.data_ptr(), scale.data_ptr(), T, d, code, _stream(x))
-    _lib.check("fsw_fp8_quantize_rows", rc)
+    _call("fsw_fp8_quantize_rows", x, x.data_ptr(), q.data_ptr(), scale.data_ptr(), T, d, code)
     return q, scale.t()
 
 
@@ -446,9 +450,7 @@ def fp8_quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     E, d_in, d_out = w.shape
     q = torch.empty((E, d_out, d_in), device=w.device, dtype=torch.float8_e4m3fn)
     scale = torch.empty((E, _blocks(d_out), _blocks(d_in)), device=w.device, dtype=torch.float32)
-    with torch.cuda.device(w.device):
-        rc = _lib.load().fsw_fp8_quantize_weight(w.data_ptr(), q.data_ptr(), scale.data_ptr(), E, d_in, d_out, code, _stream(w))
-    _lib.check("fsw_fp8_quantize_weight", rc)
+    _call("fsw_fp8_quantize_weight", w, w.data_ptr(), q.data_ptr(), scale.data_ptr(), E, d_in, d_out, code)
     return q, scale
 
 
@@ -458,10 +460,9 @@ def fp8_gemm(xq: torch.Tensor, x_scale: torch.Tensor, q: torch.Tensor, scale: to
     T, K = xq.shape
     y = torch.empty((T, q.shape[0]), device=xq.device, dtype=dtype)
     code = _code(y)
-    with torch.cuda.device(xq.device):
-        rc = _lib.load().fsw_fp8_gemm(xq.data_ptr(), x_scale.data_ptr(), x_scale.stride(0), x_scale.stride(1), q.data_ptr(),
-                                      scale.data_ptr(), y.data_ptr(), T, K, q.shape[0], code, _stream(xq))
-    _lib.check("fsw_fp8_gemm", rc)
+    _call("fsw_fp8_gemm", xq,
+          xq.data_ptr(), x_scale.data_ptr(), x_scale.stride(0), x_scale.stride(1), q.data_ptr(), scale.data_ptr(),
+          y.data_ptr(), T, K, q.shape[0], code)
     return y
 
 
@@ -474,10 +475,8 @@ def fp8_linear(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> torch.T
     nbytes = _fp8_scratch_bytes("fsw_fp8_linear_scratch_bytes", T, K)
     y = torch.empty((T, N), device=x.device, dtype=x.dtype)
     scratch = _scratch(nbytes, x)
-    with torch.cuda.device(x.device):
-        rc = _lib.load().fsw_fp8_linear(x.data_ptr(), q.data_ptr(), scale.data_ptr(), y.data_ptr(), scratch.data_ptr(), nbytes,
-                                        T, K, N, code, _stream(x))
-    _lib.check("fsw_fp8_linear", rc)
+    _call("fsw_fp8_linear", x,
+          x.data_ptr(), q.data_ptr(), scale.data_ptr(), y.data_ptr(), scratch.data_ptr(), nbytes, T, K, N, code)
     return y
 
 
@@ -489,11 +488,9 @@ def fp8_mlp(x: torch.Tensor, w_gate: torch.Tensor, s_gate: torch.Tensor, w_up: t
     nbytes = _fp8_scratch_bytes("fsw_fp8_mlp_scratch_bytes", T, d, f)
     y = torch.empty((T, d_out), device=x.device, dtype=x.dtype)
     scratch = _scratch(nbytes, x)
-    with torch.cuda.device(x.device):
-        rc = _lib.load().fsw_fp8_mlp(
-            x.data_ptr(), w_gate.data_ptr(), s_gate.data_ptr(), w_up.data_ptr(), s_up.data_ptr(), w_down.data_ptr(),
-            s_down.data_ptr(), y.data_ptr(), scratch.data_ptr(), nbytes, T, d, f, d_out, code, _stream(x))
-    _lib.check("fsw_fp8_mlp", rc)
+    _call("fsw_fp8_mlp", x,
+          x.data_ptr(), w_gate.data_ptr(), s_gate.data_ptr(), w_up.data_ptr(), s_up.data_ptr(), w_down.data_ptr(),
+          s_down.data_ptr(), y.data_ptr(), scratch.data_ptr(), nbytes, T, d, f, d_out, code)
     return y
 
 
@@ -506,10 +503,8 @@ def fp8_experts(x: torch.Tensor, weights: torch.Tensor, indices: torch.Tensor, w
     nbytes = _fp8_scratch_bytes("fsw_fp8_experts_scratch_bytes", T, k, E, d, f, d_out)
     y = torch.empty((T, d_out), device=x.device, dtype=x.dtype)
     scratch = _scratch(nbytes, x)
-    with torch.cuda.device(x.device):
-        rc = _lib.load().fsw_fp8_experts_forward(
-            x.data_ptr(), weights.data_ptr(), indices.data_ptr(), w_gate.data_ptr(), s_gate.data_ptr(), w_up.data_ptr(),
-            s_up.data_ptr(), w_down.data_ptr(), s_down.data_ptr(), y.data_ptr(), scratch.data_ptr(), nbytes, T, k, E, d, f,
-            d_out, code, _weights_code(weights, x), _stream(x))
-    _lib.check("fsw_fp8_experts_forward", rc)
+    _call("fsw_fp8_experts_forward", x,
+          x.data_ptr(), weights.data_ptr(), indices.data_ptr(), w_gate.data_ptr(), s_gate.data_ptr(), w_up.data_ptr(),
+          s_up.data_ptr(), w_down.data_ptr(), s_down.data_ptr(), y.data_ptr(), scratch.data_ptr(), nbytes, T, k, E, d,
+          f, d_out, code, _weights_code(weights, x))
     return y

@@ -273,33 +273,38 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
     denom = warp_sum(sum);
   }
   // masked experts score 0
+  const float rdenom = 1.0f / denom;
   auto score = [&](float v) {
     if (v == -INFINITY) return 0.0f;
-    return p.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - zmax) / denom;
+    return p.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - zmax) * rdenom;
   };
-  auto tolerance = [&](float v, float c) {
-    return score_tolerance(p.sigmoid != 0, score(v), v - zmax, c);
-  };
-  auto choice = [&](float v, int e) {
-    const float c = score(v) + (p.bias != nullptr ? p.bias[e] : 0.0f);
-    return v > -INFINITY && c > -INFINITY ? c : -INFINITY;
-  };
+  // The scores enter the selection only with a bias or groups.  `worst` bounds the error of
+  // every c of the row.
+  const bool by_score = p.bias != nullptr || p.groups > 1;
+  float c[EPL];
+  float worst = 0.0f;
+  if (by_score) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const int e = lane + 32 * i;
+      const float sc = score(z[i]);
+      c[i] = sc;
+      if (p.bias != nullptr && e < p.E) c[i] += p.bias[e];
+      if (z[i] > -INFINITY && c[i] > -INFINITY)
+        worst = fmaxf(worst, score_tolerance(p.sigmoid != 0, sc, z[i] - zmax, c[i]));
+      else
+        c[i] = -INFINITY;
+    }
+    worst = warp_max(worst);
+  }
 
   bool unsure = false;
   uint32_t allowed = ~0u;
   const int size = p.E / p.groups;
   if (p.groups > 1) {
-    float worst = 0.0f;  // largest error bound of a c in this row
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const int e = lane + 32 * i;
-      if (e < p.E) {
-        const float c = choice(z[i], e);
-        crow[e] = c;
-        if (c > -INFINITY) worst = fmaxf(worst, tolerance(z[i], c));
-      }
-    }
-    worst = warp_max(worst);
+    for (int i = 0; i < EPL; ++i)
+      if (lane + 32 * i < p.E) crow[lane + 32 * i] = c[i];
     __syncwarp();
     float gs;
     group_score<float>(crow, lane, p.groups, size, gs);
@@ -327,7 +332,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
     for (int i = 0; i < EPL; ++i) {
       const int e = lane + 32 * i;
       const bool eligible = e < p.E && (p.groups == 1 || ((allowed >> (e / size)) & 1u));
-      key[i] = eligible ? order_key(p.bias != nullptr ? choice(z[i], e) : z[i]) : 0u;
+      key[i] = eligible ? order_key(p.bias != nullptr ? c[i] : z[i]) : 0u;
     }
     if (p.bias == nullptr) {
       for (int j = 0; j < p.k; ++j) {
@@ -339,7 +344,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
       // Neighbours in the fp32 order must differ by more than their bounds, through the first
       // expert that is dropped.  Equal logits with equal biases tie exactly in any precision;
       // a run of them must end in a certain gap too, which is looked for a few places further.
-      float prev_c = 0.0f, prev_tol = 0.0f, prev_z = 0.0f, prev_b = 0.0f;
+      // The row's bound settles nearly all neighbours; the others are looked at one by one.
+      float prev_c = INFINITY;
+      int prev_win = 0;
       bool tie = false;
       for (int j = 0; j <= p.k + 8; ++j) {
         int win;
@@ -350,15 +357,18 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
           if (j >= p.k) break;
           continue;
         }
-        const float zc = as_f32(row[win]), b = p.bias[win], c = key_value(top);
-        const float tol = tolerance(zc, c);
-        tie = j > 0 && zc == prev_z && b == prev_b;
-        if (j > 0 && !tie && prev_c - c <= prev_tol + tol) unsure = true;
+        const float cw = key_value(top);
+        tie = false;
+        if (prev_c - cw <= 2.0f * worst) {
+          const float za = as_f32(row[prev_win]), zb = as_f32(row[win]);
+          tie = za == zb && p.bias[prev_win] == p.bias[win];
+          if (!tie)
+            unsure = prev_c - cw <= score_tolerance(p.sigmoid != 0, score(za), za - zmax, prev_c) +
+                                        score_tolerance(p.sigmoid != 0, score(zb), zb - zmax, cw);
+        }
         if (unsure || (j >= p.k && !tie)) break;
-        prev_c = c;
-        prev_tol = tol;
-        prev_z = zc;
-        prev_b = b;
+        prev_c = cw;
+        prev_win = win;
       }
       if (tie) unsure = true;
     }

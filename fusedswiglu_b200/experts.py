@@ -38,22 +38,34 @@ def check_routing(x, weights, indices):
     assert weights.dtype in (torch.float32, x.dtype), f"Expected weights in float32 or {x.dtype}, got {weights.dtype}"
 
 
+def _forward(x, weights, indices, w_gate, w_up, w_down, save):
+    """(y, saved, weights, w_gate, w_up, w_down), the last four contiguous."""
+    check_args(x, weights, indices, w_gate, w_up, w_down)
+    x2d = (x if x.ndim == 2 else x.reshape(-1, x.shape[-1])).contiguous()
+    r = (weights if weights.ndim == 2 else weights.reshape(-1, weights.shape[-1])).contiguous()
+    wg, wu, wd = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
+    y, saved = _launch.experts_forward(x2d, r, _launch.expert_indices(indices, wg.shape[0]), wg, wu, wd, save=save)
+    return (y if x.ndim == 2 else y.view(x.shape[:-1] + (wd.shape[2],)), saved, r, wg, wu, wd)
+
+
 class FusedSwiGLUExperts(Function):
     """``FusedSwiGLUExperts.apply(x, weights, indices, w_gate, w_up, w_down)``."""
 
+    @classmethod
+    def apply(cls, x, weights, indices, w_gate, w_up, w_down):
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weights, w_gate, w_up, w_down)):
+            return super().apply(x, weights, indices, w_gate, w_up, w_down)
+        # nothing to differentiate: nothing is saved, and autograd's bookkeeping is left out
+        return _forward(x, weights, indices, w_gate, w_up, w_down, False)[0]
+
     @staticmethod
     def forward(ctx, x, weights, indices, w_gate, w_up, w_down):
-        check_args(x, weights, indices, w_gate, w_up, w_down)
-        k = weights.shape[-1]
-        x2d = x.reshape(-1, x.shape[-1]).contiguous()
-        r = weights.reshape(-1, k).contiguous()
-        wg, wu, wd = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
         need = any(ctx.needs_input_grad)
-        y, saved = _launch.experts_forward(x2d, r, _launch.expert_indices(indices, wg.shape[0]), wg, wu, wd, save=need)
+        y, saved, *kept = _forward(x, weights, indices, w_gate, w_up, w_down, need)
         if need:
-            ctx.save_for_backward(r, wg, wu, wd, saved)
+            ctx.save_for_backward(*kept, saved)
         ctx.in_shape, ctx.weights_shape = x.shape, weights.shape
-        return y.view(x.shape[:-1] + (wd.shape[2],))
+        return y
 
     @staticmethod
     @once_differentiable

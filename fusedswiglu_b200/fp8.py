@@ -30,9 +30,10 @@ def _no_grad(*tensors) -> None:
 def _check_weight(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, ndim: int = 2) -> None:
     assert x.ndim >= 2 and q.ndim == ndim, "Incorrect number of dimensions"
     assert q.dtype == torch.float8_e4m3fn, f"Expected a float8_e4m3fn weight, got {q.dtype}"
-    want = q.shape[:-2] + (-(-q.shape[-2] // 128), -(-q.shape[-1] // 128))
+    *outer, n, d = q.shape
+    want = (*outer, -(-n // 128), -(-d // 128))
     assert scale.dtype == torch.float32 and scale.shape == want, (
-        f"Expected float32 scales of shape {tuple(want)}, got {scale.dtype} {tuple(scale.shape)}")
+        f"Expected float32 scales of shape {want}, got {scale.dtype} {tuple(scale.shape)}")
     assert x.shape[-1] == q.shape[-1], f"Dimension mismatch. Expected x.shape[-1] ({x.shape[-1]}) to be equal to the weight's inner size ({q.shape[-1]})"
 
 
@@ -76,6 +77,8 @@ def fp8_linear(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> torch.T
     """y (..., d_out) in x's type: x (..., d_in), bf16 or fp16, times a quantised weight."""
     _no_grad(x)
     _check_weight(x, q, scale)
+    if x.ndim == 2:
+        return _launch.fp8_linear(x.contiguous(), q.contiguous(), scale.contiguous())
     x2d = x.reshape(-1, x.shape[-1]).contiguous()
     return _launch.fp8_linear(x2d, q.contiguous(), scale.contiguous()).view(x.shape[:-1] + (q.shape[0],))
 

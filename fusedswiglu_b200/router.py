@@ -16,8 +16,21 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import _launch
+
+
+def _forward(logits, bias, top_k, score, renormalize, scale, num_groups, topk_groups):
+    assert logits.ndim >= 2, "Expected logits of shape (..., num_experts)"
+    assert score in ("softmax", "sigmoid"), f"Expected score 'softmax' or 'sigmoid', got {score!r}"
+    E = logits.shape[-1]
+    if bias is not None:
+        assert bias.shape == (E,), f"Expected a bias of shape ({E},), got {tuple(bias.shape)}"
+    z = logits.reshape(-1, E) if logits.ndim != 2 else logits
+    if z.stride(1) != 1 or (z.shape[0] > 1 and z.stride(0) < E):
+        z = z.contiguous()
+    return (z, *_launch.route(z, bias, int(top_k), score, bool(renormalize), float(scale), int(num_groups), int(topk_groups)))
 
 
 class FusedRouter(Function):
@@ -26,16 +39,7 @@ class FusedRouter(Function):
 
     @staticmethod
     def forward(ctx, logits, bias, top_k, score, renormalize, scale, num_groups, topk_groups):
-        assert logits.ndim >= 2, "Expected logits of shape (..., num_experts)"
-        assert score in ("softmax", "sigmoid"), f"Expected score 'softmax' or 'sigmoid', got {score!r}"
-        E = logits.shape[-1]
-        if bias is not None:
-            assert bias.shape == (E,), f"Expected a bias of shape ({E},), got {tuple(bias.shape)}"
-        z = logits.reshape(-1, E)
-        if z.stride(1) != 1 or (z.shape[0] > 1 and z.stride(0) < E):
-            z = z.contiguous()
-        weights, indices = _launch.route(z, bias, int(top_k), score, bool(renormalize), float(scale),
-                                         int(num_groups), int(topk_groups))
+        z, weights, indices = _forward(logits, bias, top_k, score, renormalize, scale, num_groups, topk_groups)
         ctx.save_for_backward(z, indices)
         ctx.args = (score, bool(renormalize), float(scale))
         ctx.in_shape = logits.shape
@@ -45,6 +49,7 @@ class FusedRouter(Function):
         return weights.view(shape), out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_weights, _grad_indices):
         dz = None
         if ctx.needs_input_grad[0]:
@@ -63,4 +68,11 @@ def route(logits: torch.Tensor, top_k: int, *, bias: Optional[torch.Tensor] = No
 
     At most 1024 experts, 32 of them per token, 32 groups of equal size.  ``bias``: one
     value per expert, added to the scores for the selection only."""
-    return FusedRouter.apply(logits, bias, top_k, score, renormalize, scale, num_groups, topk_groups)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return FusedRouter.apply(logits, bias, top_k, score, renormalize, scale, num_groups, topk_groups)
+    # nothing to differentiate: autograd's bookkeeping costs more than the kernel
+    _, weights, indices = _forward(logits, bias, top_k, score, renormalize, scale, num_groups, topk_groups)
+    if logits.ndim != 2:
+        shape = logits.shape[:-1] + (int(top_k),)
+        weights, indices = weights.view(shape), indices.view(shape)
+    return weights, indices
