@@ -39,6 +39,7 @@ struct RouteParams {
   int E, k, groups, topk_groups;
   int sigmoid, renorm;
   float scale;
+  uint32_t group_magic;  // e / (E / groups) = umulhi(e, group_magic) for e < 1024; 0: groups of one
 };
 
 template <typename T>
@@ -93,7 +94,11 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
 // Largest key of the warp; ties to the lowest index.
 __device__ __forceinline__ uint32_t warp_best(uint32_t key, int index, int& winner) {
   const uint32_t top = __reduce_max_sync(kFull, key);
-  winner = static_cast<int>(__reduce_min_sync(kFull, key == top ? static_cast<unsigned>(index) : 0x7fffffffu));
+  const unsigned lanes = __ballot_sync(kFull, key == top);
+  if ((lanes & (lanes - 1u)) == 0u)  // one lane, nearly always: a vote and a shuffle, not a second reduction
+    winner = __shfl_sync(kFull, index, __ffs(lanes) - 1);
+  else
+    winner = static_cast<int>(__reduce_min_sync(kFull, key == top ? static_cast<unsigned>(index) : 0x7fffffffu));
   return top;
 }
 __device__ __forceinline__ unsigned long long warp_best(unsigned long long key, int index, int& winner) {
@@ -110,23 +115,60 @@ __device__ __forceinline__ unsigned long long warp_best(unsigned long long key, 
   return key;
 }
 
-// The next pick among the lane's keys; the winner's key is cleared.
-template <int EPL, typename K>
-__device__ __forceinline__ K take_best(K (&key)[EPL], int lane, int& winner) {
-  K best = key[0];
-  int at = lane;
+// A run of picks among the lanes' keys: each lane keeps its two best at hand, and looks through its
+// keys for the next one only when it has given both.
+template <int EPL>
+struct Picker {
+  uint32_t (&key)[EPL];
+  int lane;
+  uint32_t first = 0u, second = 0u, taken = 0u;  // taken: keys of this lane already picked
+  int first_at = 0, second_at = 0;
+  bool have_second = true;
+
+  __device__ __forceinline__ Picker(uint32_t (&k)[EPL], int l) : key(k), lane(l) {
 #pragma unroll
-  for (int i = 1; i < EPL; ++i)
-    if (key[i] > best) {
-      best = key[i];
-      at = lane + 32 * i;
+    for (int i = 0; i < EPL; ++i) {
+      if (key[i] > first) {  // strict: of equal keys the lowest index comes first
+        second = first;
+        second_at = first_at;
+        first = key[i];
+        first_at = i;
+      } else if (key[i] > second) {
+        second = key[i];
+        second_at = i;
+      }
     }
-  const K top = warp_best(best, at, winner);
+  }
+
+  __device__ __forceinline__ uint32_t take(int& winner) {
+    const uint32_t top = warp_best(first, lane + 32 * first_at, winner);
+    bool again = false;
+    if ((winner & 31) == lane) {
+      taken |= 1u << first_at;
+      again = !have_second;
+      first = second;
+      first_at = second_at;
+      have_second = false;
+    }
+    if (__any_sync(kFull, again)) {
+      uint32_t best = 0u;
+      int at = 0;
 #pragma unroll
-  for (int i = 0; i < EPL; ++i)
-    if (lane + 32 * i == winner) key[i] = 0;
-  return top;
-}
+      for (int i = 0; i < EPL; ++i) {
+        const uint32_t k = ((taken >> i) & 1u) ? 0u : key[i];
+        if (k > best) {
+          best = k;
+          at = i;
+        }
+      }
+      if (again) {
+        first = best;
+        first_at = at;
+      }
+    }
+    return top;
+  }
+};
 
 // Sum of the two largest c of group `lane / lanes_per_group`, from the warp's row of c in
 // shared memory.  Masked experts hold -inf and add nothing; a group of only such scores -inf.
@@ -139,21 +181,13 @@ __device__ __forceinline__ void group_score(const F* c, int lane, int groups, in
   if (g < groups)
     for (int j = r; j < size; j += lpg) {
       const F v = c[g * size + j];
-      if (v > m1) {
-        m2 = m1;
-        m1 = v;
-      } else if (v > m2) {
-        m2 = v;
-      }
+      m2 = max(m2, min(m1, v));
+      m1 = max(m1, v);
     }
   for (int o = lpg >> 1; o > 0; o >>= 1) {
     const F a = __shfl_xor_sync(kFull, m1, o), b = __shfl_xor_sync(kFull, m2, o);
-    if (a > m1) {
-      m2 = m1 > b ? m1 : b;
-      m1 = a;
-    } else if (a > m2) {
-      m2 = a;
-    }
+    m2 = max(max(m2, b), min(m1, a));
+    m1 = max(m1, a);
   }
   // lane g of the result (all lanes of a group agree)
   const F sum = (m2 > low) ? m1 + m2 : m1;
@@ -161,65 +195,76 @@ __device__ __forceinline__ void group_score(const F* c, int lane, int groups, in
   if (lane >= groups) score = low;
 }
 
-// Error bound of an fp32 score s = exp(d) / sum or 1 / (1 + exp(-z)), |d| the magnitude of
-// the argument's rounding, and of c = s + bias, in units of 2^-23: 8 cover exp, the addition
-// and the division; a softmax adds up to 40 from the sum of the row and |d| from the rounded
-// difference z - max.
-__device__ __forceinline__ float score_tolerance(bool sigmoid, float s, float d, float c) {
-  return 1.2e-7f * (s * (sigmoid ? 8.0f : fabsf(d) + 64.0f) + fabsf(c)) + 1e-37f;
+// Error bound of a score as route_kernel computes it for the selection, and of c = s + bias, in
+// units of 2^-23.  The exponential by ex2.approx is good to a few units and |argument| roundings
+// of 2^-24 each; sigmoid: s changes by s (1 - s) of that, plus the sum and the reciprocal: 8 + |z|
+// units of s cover it.  softmax: up to 40 roundings from the sum of the row, and the rounded
+// difference d = z - max: 64 + |d| units of s.
+__device__ __forceinline__ float score_tolerance(bool sigmoid, float s, float arg, float c) {
+  return 1.2e-7f * (s * (fabsf(arg) + (sigmoid ? 8.0f : 64.0f)) + fabsf(c)) + 1e-37f;
 }
 
-// Scores of a row in 64 bits, and the selection from them: lane j gets pick j.
-// Runs for the few rows whose fp32 order is not certain.
-template <typename T, int EPL>
-__device__ __noinline__ int select64(const RouteParams& p, const T* row, float zmax, double* crow, int lane) {
-  double c[EPL];
+// The selection from scores in 64 bits: lane j gets pick j.  Runs for the few rows whose fp32
+// order is not certain; small rather than fast (loops, the row's keys in shared memory), so
+// that it costs the other rows neither registers nor instruction cache.
+template <typename T>
+__device__ __noinline__ int select64(const RouteParams& p, const T* row, float zmax, double* c, int lane) {
   double sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
-    const float z = e < p.E ? as_f32(row[e]) : -INFINITY;
-    c[i] = p.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(z))) : exp(static_cast<double>(z) - static_cast<double>(zmax));
-    sum += c[i];
+  if (!p.sigmoid) {
+#pragma unroll 1
+    for (int e = lane; e < p.E; e += 32) {
+      const float z = as_f32(row[e]);
+      if (z != -INFINITY) sum += exp(static_cast<double>(z) - static_cast<double>(zmax));
+    }
+    sum = warp_sum(sum);
   }
-  if (!p.sigmoid) sum = warp_sum(sum);
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
-    const float z = e < p.E ? as_f32(row[e]) : -INFINITY;
-    if (!p.sigmoid) c[i] /= sum;
-    if (p.bias != nullptr && e < p.E) c[i] += static_cast<double>(p.bias[e]);
-    if (!(z > -INFINITY) || !(c[i] > -INFINITY)) c[i] = -INFINITY;
-    if (p.groups > 1 && e < p.E) crow[e] = c[i];
+#pragma unroll 1
+  for (int e = lane; e < p.E; e += 32) {
+    const float z = as_f32(row[e]);
+    const double d = exp(p.sigmoid ? -static_cast<double>(z) : static_cast<double>(z) - static_cast<double>(zmax));
+    double v = p.sigmoid ? 1.0 / (1.0 + d) : d / sum;
+    if (p.bias != nullptr) v += static_cast<double>(p.bias[e]);
+    c[e] = (z > -INFINITY && v > -INFINITY) ? v : -INFINITY;
   }
-  unsigned long long allowed = ~0ull;
+  __syncwarp();
+  uint32_t allowed = ~0u;
   const int size = p.E / p.groups;
   if (p.groups > 1) {
-    __syncwarp();
     double gs;
-    group_score<double>(crow, lane, p.groups, size, gs);
-    unsigned long long key[1] = {lane < p.groups ? order_key(gs) : 0ull};
-    allowed = 0ull;
+    group_score<double>(c, lane, p.groups, size, gs);
+    unsigned long long key = lane < p.groups ? order_key(gs) : 0ull;
+    allowed = 0u;
+#pragma unroll 1
     for (int j = 0; j < p.topk_groups; ++j) {
       int win;
-      take_best<1>(key, lane, win);
-      allowed |= 1ull << win;
+      warp_best(key, lane, win);
+      if (win == lane) key = 0ull;
+      allowed |= 1u << win;
     }
     __syncwarp();
   }
-  unsigned long long key[EPL];
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
-    const double v = p.bias != nullptr ? c[i] : (e < p.E ? static_cast<double>(as_f32(row[e])) : -INFINITY);
-    key[i] = (e < p.E && ((allowed >> (e / size & 63)) & 1ull)) ? order_key(v) : 0ull;
+  unsigned long long* key = reinterpret_cast<unsigned long long*>(c);
+#pragma unroll 1
+  for (int e = lane; e < p.E; e += 32) {
+    const double v = p.bias != nullptr ? c[e] : static_cast<double>(as_f32(row[e]));
+    key[e] = (p.groups == 1 || ((allowed >> (e / size)) & 1u)) ? order_key(v) : 0ull;
   }
   int mine = 0;
+#pragma unroll 1
   for (int j = 0; j < p.k; ++j) {
-    int win;
-    take_best<EPL>(key, lane, win);
+    unsigned long long best = 0ull;
+    int at = lane, win;
+#pragma unroll 1
+    for (int e = lane; e < p.E; e += 32)  // each lane reads and clears only its own keys
+      if (key[e] > best) {
+        best = key[e];
+        at = e;
+      }
+    warp_best(best, at, win);
+    if ((win & 31) == lane) key[win] = 0ull;
     if (lane == j) mine = win;
   }
+  __syncwarp();
   return mine;
 }
 
@@ -246,16 +291,15 @@ __device__ __forceinline__ float pick_share(const RouteParams& p, float z, int l
 }
 
 // One warp per token.  EPL = experts per lane (a power of two, 32 * EPL >= E).
-template <typename T, int EPL>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteParams p) {
+template <typename T, int EPL, bool SIGMOID, bool BIAS, bool GROUPS>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_constant__ RouteParams p) {
   extern __shared__ double route_smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double* crow64 = route_smem + static_cast<size_t>(warp) * p.E;  // with a bias or groups only
+  float* crow = reinterpret_cast<float*>(crow64);
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
   if (t >= p.T) return;
-  double* crow64 = route_smem + static_cast<size_t>(warp) * p.E;  // groups > 1 only
-  float* crow = reinterpret_cast<float*>(crow64);
   const T* row = static_cast<const T*>(p.logits) + t * p.ld;
-
   float z[EPL];
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
@@ -263,7 +307,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
     z[i] = e < p.E ? as_f32(row[e]) : -INFINITY;
   }
   float zmax = -INFINITY, denom = 1.0f;
-  if (!p.sigmoid) {
+  if (!SIGMOID) {
 #pragma unroll
     for (int i = 0; i < EPL; ++i) zmax = fmaxf(zmax, z[i]);
     zmax = warp_max(zmax);
@@ -272,49 +316,48 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
     for (int i = 0; i < EPL; ++i) sum += z[i] == -INFINITY ? 0.0f : expf(z[i] - zmax);  // NaN and +inf make it NaN
     denom = warp_sum(sum);
   }
-  // masked experts score 0
-  const float rdenom = 1.0f / denom;
-  auto score = [&](float v) {
-    if (v == -INFINITY) return 0.0f;
-    return p.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - zmax) * rdenom;
+  const float rdenom = 1.0f / denom, base = zmax > -INFINITY ? zmax : 0.0f;
+  auto score = [&](float v) {  // -inf scores 0
+    return SIGMOID ? __fdividef(1.0f, 1.0f + __expf(-v)) : __expf(v - base) * rdenom;
   };
   // The scores enter the selection only with a bias or groups.  `worst` bounds the error of
-  // every c of the row.
-  const bool by_score = p.bias != nullptr || p.groups > 1;
+  // every c of the row: s (8 + |z|) <= 18 where that bound is near the truth (z <= 10; beyond
+  // it s is 1 to the last bits), and s (64 + |d|) <= 66 max s.
+  constexpr bool by_score = BIAS || GROUPS;
   float c[EPL];
   float worst = 0.0f;
-  if (by_score) {
+  if constexpr (by_score) {
+    float largest = 0.0f;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
       const int e = lane + 32 * i;
-      const float sc = score(z[i]);
-      c[i] = sc;
-      if (p.bias != nullptr && e < p.E) c[i] += p.bias[e];
-      if (z[i] > -INFINITY && c[i] > -INFINITY)
-        worst = fmaxf(worst, score_tolerance(p.sigmoid != 0, sc, z[i] - zmax, c[i]));
-      else
-        c[i] = -INFINITY;
+      c[i] = score(z[i]);
+      if (BIAS && e < p.E) c[i] += p.bias[e];
+      const bool open = z[i] > -INFINITY && c[i] > -INFINITY;  // neither -inf nor NaN
+      largest = fmaxf(largest, open ? fabsf(c[i]) : 0.0f);
+      c[i] = open ? c[i] : -INFINITY;
     }
-    worst = warp_max(worst);
+    worst = 1.2e-7f * ((SIGMOID ? 18.0f : 66.0f * rdenom) + warp_max(largest)) + 1e-37f;
   }
 
   bool unsure = false;
   uint32_t allowed = ~0u;
-  const int size = p.E / p.groups;
-  if (p.groups > 1) {
+  const int size = GROUPS ? p.E / p.groups : p.E;
+  if constexpr (GROUPS) {
 #pragma unroll
     for (int i = 0; i < EPL; ++i)
       if (lane + 32 * i < p.E) crow[lane + 32 * i] = c[i];
     __syncwarp();
     float gs;
     group_score<float>(crow, lane, p.groups, size, gs);
-    uint32_t key[1] = {lane < p.groups ? order_key(gs) : 0u};
+    uint32_t key = lane < p.groups ? order_key(gs) : 0u;
     allowed = 0u;
     uint32_t prev = 0u;
     const int rounds = p.topk_groups < p.groups ? p.topk_groups + 1 : p.topk_groups;
     for (int j = 0; j < rounds; ++j) {
       int win;
-      const uint32_t top = take_best<1>(key, lane, win);
+      const uint32_t top = warp_best(key, lane, win);
+      if (win == lane) key = 0u;
       if (j < p.topk_groups) allowed |= 1u << win;
       // only the border between kept and dropped groups matters; sums of two: two bounds each,
       // and the rounding of the sums
@@ -331,13 +374,15 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
       const int e = lane + 32 * i;
-      const bool eligible = e < p.E && (p.groups == 1 || ((allowed >> (e / size)) & 1u));
-      key[i] = eligible ? order_key(p.bias != nullptr ? c[i] : z[i]) : 0u;
+      const uint32_t g = p.group_magic ? __umulhi(e, p.group_magic) : e;
+      const bool eligible = e < p.E && (!GROUPS || ((allowed >> (g & 31u)) & 1u));
+      key[i] = eligible ? order_key(BIAS ? c[i] : z[i]) : 0u;
     }
-    if (p.bias == nullptr) {
+    Picker<EPL> picker(key, lane);
+    if constexpr (!BIAS) {
       for (int j = 0; j < p.k; ++j) {
         int win;
-        take_best<EPL>(key, lane, win);
+        picker.take(win);
         if (lane == j) mine = win;
       }
     } else {
@@ -350,7 +395,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
       bool tie = false;
       for (int j = 0; j <= p.k + 8; ++j) {
         int win;
-        const uint32_t top = take_best<EPL>(key, lane, win);
+        const uint32_t top = picker.take(win);
         if (j < p.k && lane == j) mine = win;
         if (top <= 1u) {  // from here on only masked experts, which rank by index, or none
           tie = false;
@@ -363,8 +408,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
           const float za = as_f32(row[prev_win]), zb = as_f32(row[win]);
           tie = za == zb && p.bias[prev_win] == p.bias[win];
           if (!tie)
-            unsure = prev_c - cw <= score_tolerance(p.sigmoid != 0, score(za), za - zmax, prev_c) +
-                                        score_tolerance(p.sigmoid != 0, score(zb), zb - zmax, cw);
+            unsure = prev_c - cw <= score_tolerance(SIGMOID, score(za), SIGMOID ? za : za - base, prev_c) +
+                                        score_tolerance(SIGMOID, score(zb), SIGMOID ? zb : zb - base, cw);
         }
         if (unsure || (j >= p.k && !tie)) break;
         prev_c = cw;
@@ -373,16 +418,16 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
       if (tie) unsure = true;
     }
   }
-  if (unsure) mine = select64<T, EPL>(p, row, zmax, crow64, lane);
+  if (by_score && unsure) mine = select64<T>(p, row, zmax, crow64, lane);
 
   const float zp = lane < p.k ? as_f32(row[mine]) : -INFINITY;
   float w;
   if (p.renorm) {
     w = pick_share(p, zp, lane);
-    if (!p.sigmoid && !(denom == denom)) w = denom;  // a NaN or +inf in a softmax row: NaN
+    if (!SIGMOID && !(denom == denom)) w = denom;  // a NaN or +inf in a softmax row: NaN
   } else {
-    w = score(zp);
-    if (!p.sigmoid && zp == -INFINITY && !(denom == denom)) w = denom;
+    w = zp == -INFINITY ? 0.0f : SIGMOID ? 1.0f / (1.0f + expf(-zp)) : expf(zp - zmax) / denom;
+    if (!SIGMOID && zp == -INFINITY && !(denom == denom)) w = denom;
   }
   if (lane < p.k) {
     p.weights[t * p.k + lane] = w * p.scale;
@@ -461,17 +506,34 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_backward_kernel(const 
   }
 }
 
+// What a call does not ask for is not in its kernel: the tests of it per expert cost as much
+// as the selection.
+template <typename T, int EPL, bool SIGMOID>
+void launch_kind(const RouteParams& p, unsigned blocks, size_t smem, cudaStream_t st) {
+  auto* kernel = p.bias != nullptr
+                     ? (p.groups > 1 ? route_kernel<T, EPL, SIGMOID, true, true> : route_kernel<T, EPL, SIGMOID, true, false>)
+                     : (p.groups > 1 ? route_kernel<T, EPL, SIGMOID, false, true> : route_kernel<T, EPL, SIGMOID, false, false>);
+  kernel<<<blocks, kRouteWarps * 32, smem, st>>>(p);
+}
+template <typename T, int EPL>
+void launch_forward(const RouteParams& p, unsigned blocks, size_t smem, cudaStream_t st) {
+  if (p.sigmoid)
+    launch_kind<T, EPL, true>(p, blocks, smem, st);
+  else
+    launch_kind<T, EPL, false>(p, blocks, smem, st);
+}
+
 template <typename T>
 cudaError_t launch_route(const RouteParams& p, bool backward, cudaStream_t st) {
   const unsigned blocks = static_cast<unsigned>((p.T + kRouteWarps - 1) / kRouteWarps);
-  const size_t smem = (!backward && p.groups > 1) ? static_cast<size_t>(kRouteWarps) * p.E * sizeof(double) : 0;
+  const size_t smem = (!backward && (p.groups > 1 || p.bias != nullptr)) ? static_cast<size_t>(kRouteWarps) * p.E * sizeof(double) : 0;
   ++g_kernel_launches;
 #define FSW_ROUTE(EPL)                                                         \
   if (p.E <= 32 * EPL) {                                                       \
     if (backward)                                                              \
       route_backward_kernel<T, EPL><<<blocks, kRouteWarps * 32, 0, st>>>(p);   \
     else                                                                       \
-      route_kernel<T, EPL><<<blocks, kRouteWarps * 32, smem, st>>>(p);         \
+      launch_forward<T, EPL>(p, blocks, smem, st);                             \
     return cudaGetLastError();                                                 \
   }
   FSW_ROUTE(1)
@@ -531,6 +593,8 @@ int fsw_route(const void* logits, int64_t ld, const void* bias, void* weights, v
   p.sigmoid = score == FSW_SCORE_SIGMOID;
   p.renorm = renormalize != 0;
   p.scale = scale;
+  const unsigned size = (unsigned)(E / num_groups);
+  p.group_magic = size > 1 ? (uint32_t)(((1ull << 32) + size - 1) / size) : 0u;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == FSW_BF16)
     FSW_CUDA(launch_route<__nv_bfloat16>(p, false, st));
