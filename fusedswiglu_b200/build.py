@@ -16,7 +16,7 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_NAME = "libfused_swiglu_sm100.so"
 LIB_PATH = PKG_DIR / LIB_NAME
-SOURCES = [CSRC / "fsw_api.cu", CSRC / "fsw_route.cu", CSRC / "fsw_experts.cu", CSRC / "fsw_fp8.cu"]
+SOURCES = [CSRC / "fsw_api.cu", CSRC / "fsw_route.cu", CSRC / "fsw_experts.cu", CSRC / "fsw_few.cu", CSRC / "fsw_fp8.cu"]
 PUBLIC_HEADER = PKG_DIR.parent / "include" / "fused_swiglu.h"
 HEADERS = [CSRC / "fsw_ptx.cuh", CSRC / "fsw_gemm.cuh", CSRC / "fsw_host.h", CSRC / "fsw_experts.h", PUBLIC_HEADER]
 OBJ_DIR = CSRC / "build"

@@ -667,6 +667,9 @@ int fsw_experts_forward(const void* x, const void* weights, const void* indices,
   x_.dtype = dtype;
   x_.cg = x_.plan.tile_rows / 128;
   x_.st = static_cast<cudaStream_t>(stream);
+  if (!train && few_rows_apply(T, k, d, f, x_.dev->sm_count) && scratch_bytes >= T * k * f * 4)
+    return experts_few_rows(x, weights, weights_dtype, static_cast<const int*>(indices), w_gate, w_up, w_down, y,
+                            static_cast<float*>(scratch), T, k, E, d, f, d_out, dtype, x_.dev, x_.st);
   char* keep = static_cast<char*>(train ? saved : scratch);
   char* tmp = static_cast<char*>(scratch) + (train ? 0 : b.g);
   int* plan = reinterpret_cast<int*>(keep);

@@ -67,6 +67,13 @@ int gather_rows(const ExpertPlan& p, const int* plan, const void* src, void* dst
 int combine_rows(const ExpertPlan& p, const int* plan, const void* src, const void* weights, int wtype, void* y,
                  int64_t cols, int dtype, cudaStream_t st);
 
+// The forward for a handful of tokens without the sort and the matrix kernels (fsw_few.cu);
+// h: T * k * f floats of scratch.
+bool few_rows_apply(int64_t T, int k, int64_t d, int64_t f, int sms);
+int experts_few_rows(const void* x, const void* weights, int wtype, const int* indices, const void* w_gate, const void* w_up,
+                     const void* w_down, void* y, float* h, int64_t T, int k, int E, int64_t d, int64_t f, int64_t d_out,
+                     int dtype, DeviceInfo* dev, cudaStream_t st);
+
 int check_experts(int64_t T, int k, int E, int64_t d, int64_t f, int64_t d_out, int dtype, int wtype);
 
 }  // namespace fsw

@@ -234,3 +234,29 @@ def test_moe_block_router_and_experts_together(score):
     for name, a, b in zip(("x", "router", "gate", "up", "down"), got, want):
         # the logits' rounding (half a step of values up to 3) moves a weight by that much too
         assert rel(a, b) < 3 * HALF[torch.bfloat16], (name, rel(a, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,E,k,d,f,o", [(1, 1, 1, 8, 8, 8), (1, 64, 32, 136, 72, 40), (4, 8, 8, 1032, 264, 520),
+                                        (2, 3, 2, 4096, 136, 2056), (3, 16, 4, 520, 1408, 1024), (4, 6, 1, 256, 128, 264)])
+def test_a_handful_of_tokens(T, E, k, d, f, o, dtype):
+    """Inference on up to four tokens: fp32 and 16-bit weights, dropped pairs, repeated experts."""
+    for wdtype in (torch.float32, dtype):
+        x, w, idx, wg, wu, wd, _ = inputs(T, E, k, d, f, o, dtype, seed=T + k, wdtype=wdtype)
+        compare(run(x, w, idx, wg, wu, wd), definition(x, w, idx, wg, wu, wd), dtype)
+        idx[0, k // 2] = -1 if k > 1 else E
+        idx[-1] = int(idx[-1, 0])
+        wg[0, 0] = math.nan if k > 1 else 0.0
+        keep = (idx != 0).all(dim=1)
+        got, want = run(x, w, idx, wg, wu, wd), definition(x, w, idx, wg, wu, wd)
+        compare([got[0][keep]], [want[0][keep]], dtype)
+
+
+def test_the_number_of_tokens_does_not_change_a_token():
+    """The same tokens alone and among others, through the forms for few and for many rows: apart
+    by the roundings of the second, not by more."""
+    x, w, idx, wg, wu, wd, _ = inputs(64, 8, 2, 256, 136, 256, torch.bfloat16, seed=20)
+    many = run(x, w, idx, wg, wu, wd)[0]
+    for T in (1, 3, 4, 5, 16):
+        few = run(x[:T], w[:T], idx[:T], wg, wu, wd)[0]
+        assert rel(few, many[:T].double()) < 3 * HALF[torch.bfloat16]
