@@ -4,21 +4,21 @@
 //   plan      sort the (token, expert) pairs by expert           (fsw_experts.h)
 //   gather    xs[row] = x[token]
 //   GFWD      h = silu(xs Wg_e) * (xs Wu_e)        one dual GEMM over all experts
-//   GNN       ys = h Wd_e
+//   GNN       ys = h Wd_e                          fp32
 //   combine   y_t = sum_j w_tj ys[row of (t, j)]   fp32, fixed order, one rounding
 // backward
 //   gather    dys[row] = dy[token]
-//   GNT       dh = dys Wd_e^T
+//   GNT       dh = dys Wd_e^T                      fp32
 //   gate      dw_tj = <h, dh>;  dg, du from w dh;  hs = w h
 //   GTN       dWd_e = hs^T dys
-//   GDX       dxs = dg Wg_e^T + du Wu_e^T
+//   GDX       dxs = dg Wg_e^T + du Wu_e^T          fp32
 //   GDW       dWg_e, dWu_e = xs^T [dg | du]
 //   combine   dx_t = sum_j dxs[row of (t, j)]
 //
 // The products are the tcgen05 kernel of fsw_gemm.cuh; what each is bound by stands in
-// DESIGN's table.  Every intermediate is rounded to the tensors' 16-bit type once, when it
-// becomes an operand of the next product (the tensor cores take 16-bit operands); sums,
-// the gate and the combination are fp32.  Nothing is summed with atomics: results do not
+// DESIGN's table.  What becomes an operand of the next product (h, hs, dg, du) is rounded to the
+// tensors' 16-bit type once, there (the tensor cores take 16-bit operands); g, u, dh, ys and
+// dxs, the gate and the sums are fp32.  Nothing is summed with atomics: results do not
 // depend on the order of execution.
 #include <cstring>
 
@@ -225,10 +225,12 @@ __device__ __forceinline__ float weight_value(const void* w, int64_t i) {
   else return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
 }
 
-template <typename T, typename W, bool WEIGHTED>
+// S: type of the rows, T or float.
+template <typename T, typename W, bool WEIGHTED, typename S>
 __global__ void __launch_bounds__(128) combine_kernel(const ExpertPlan p, const int* __restrict__ plan,
                                                       const uint4* __restrict__ src, const void* __restrict__ weights,
                                                       uint4* __restrict__ y, int vecs) {
+  constexpr int PARTS = sizeof(S) / 2;  // 16-byte vectors that 8 columns take
   ptx::allow_successor();
   ptx::wait_predecessor();
   const int64_t t = blockIdx.x;
@@ -238,25 +240,31 @@ __global__ void __launch_bounds__(128) combine_kernel(const ExpertPlan p, const 
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
     for (int j0 = 0; j0 < p.k; j0 += 4) {
-      uint4 x[4];
+      uint4 x[4][PARTS];
       float w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = j0 + j < p.k ? rows[j0 + j] : -1;
         w[j] = 0.0f;
-        x[j] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int h = 0; h < PARTS; ++h)
+          x[j][h] = r >= 0 ? ld_stream(src + (static_cast<int64_t>(r) * vecs + v) * PARTS + h) : make_uint4(0u, 0u, 0u, 0u);
         if (r >= 0) {
-          x[j] = ld_stream(src + static_cast<int64_t>(r) * vecs + v);
           w[j] = WEIGHTED ? weight_value<W>(weights, t * p.k + j0 + j) : 1.0f;
         }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t* q = reinterpret_cast<const uint32_t*>(&x[j]);
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(&x[j][0]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float lo, hi;
-          unpack2<T>(q[i], lo, hi);
+          if constexpr (PARTS == 2) {
+            lo = __uint_as_float(q[2 * i]);
+            hi = __uint_as_float(q[2 * i + 1]);
+          } else {
+            unpack2<T>(q[i], lo, hi);
+          }
           acc[2 * i] = fmaf(w[j], lo, acc[2 * i]);
           acc[2 * i + 1] = fmaf(w[j], hi, acc[2 * i + 1]);
         }
@@ -272,15 +280,15 @@ __global__ void __launch_bounds__(128) combine_kernel(const ExpertPlan p, const 
 }
 
 // -------------------------------------------------------- gate and weights --
-// One block per row.  h = silu(g) u from the saved 16-bit g and u;
-// dw = <h, dh>;  with d = w dh:  du = d silu(g), dg = d u silu'(g);  hs = w h.
-// dg overwrites dh.  Rows of the padding get zeros, whatever the weights held.
+// One block per row.  h = silu(g) u;  dw = <h, dh>;  with d = w dh:  du = d silu(g),
+// dg = d u silu'(g);  hs = w h.  fp32 in, 16-bit operands out.
+// Rows of the padding get zeros, whatever the weights held.
 template <typename T, typename W>
 __global__ void __launch_bounds__(256) expert_gate_kernel(const ExpertPlan p, const int* __restrict__ plan,
-                                                          uint4* dh, const uint4* __restrict__ g,
-                                                          const uint4* __restrict__ u, const void* __restrict__ weights,
-                                                          uint4* __restrict__ du, uint4* __restrict__ hs,
-                                                          void* dweights, int vecs) {
+                                                          const float4* __restrict__ dh, const float4* __restrict__ g,
+                                                          const float4* __restrict__ u, const void* __restrict__ weights,
+                                                          uint2* __restrict__ dg, uint2* __restrict__ du,
+                                                          uint2* __restrict__ hs, void* dweights, int vecs) {
   ptx::allow_successor();
   ptx::wait_predecessor();
   const int64_t row = blockIdx.x;
@@ -288,37 +296,45 @@ __global__ void __launch_bounds__(256) expert_gate_kernel(const ExpertPlan p, co
   const int pair = plan[p.row_pair + row];
   const float w = pair >= 0 ? weight_value<W>(weights, pair) : 0.0f;
   float dot = 0.0f;
-  for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-    const int64_t at = row * vecs + v;
-    uint4 odg = make_uint4(0u, 0u, 0u, 0u), odu = odg, ohs = odg;
-    if (pair >= 0) {
-      const uint4 vd = dh[at], vg = ld_stream(g + at), vu = ld_stream(u + at);
-      const uint32_t *wd = reinterpret_cast<const uint32_t*>(&vd), *wg = reinterpret_cast<const uint32_t*>(&vg),
-                     *wu = reinterpret_cast<const uint32_t*>(&vu);
-      uint32_t *pg = reinterpret_cast<uint32_t*>(&odg), *pu = reinterpret_cast<uint32_t*>(&odu),
-               *ph = reinterpret_cast<uint32_t*>(&ohs);
+  constexpr int kUnroll = 2;  // both vectors' loads in flight together
+  for (int v0 = threadIdx.x; v0 < vecs; v0 += kUnroll * blockDim.x) {
+    float4 vd[kUnroll], vg[kUnroll], vu[kUnroll];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float d2[2], g2[2], u2[2], rg[2], ru[2], rh[2];
-        unpack2<T>(wd[i], d2[0], d2[1]);
-        unpack2<T>(wg[i], g2[0], g2[1]);
-        unpack2<T>(wu[i], u2[0], u2[1]);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float s = sigmoid_f32(g2[c]), silu = g2[c] * s, h = silu * u2[c], d = w * d2[c];
-          dot = fmaf(h, d2[c], dot);
-          ru[c] = d * silu;
-          rg[c] = d * u2[c] * fmaf(silu, 1.0f - s, s);
-          rh[c] = w * h;
-        }
-        pg[i] = pack2<T>(rg[0], rg[1]);
-        pu[i] = pack2<T>(ru[0], ru[1]);
-        ph[i] = pack2<T>(rh[0], rh[1]);
+    for (int i = 0; i < kUnroll; ++i) {
+      const int v = v0 + i * blockDim.x;
+      if (pair >= 0 && v < vecs) {
+        const int64_t at = row * vecs + v;
+        vd[i] = __ldcs(dh + at);
+        vg[i] = __ldcs(g + at);
+        vu[i] = __ldcs(u + at);
       }
     }
-    dh[at] = odg;
-    du[at] = odu;
-    if (hs != nullptr) hs[at] = ohs;
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int v = v0 + i * blockDim.x;
+      if (v >= vecs) continue;
+      uint2 odg = make_uint2(0u, 0u), odu = odg, ohs = odg;
+      if (pair >= 0) {
+        const float d4[4] = {vd[i].x, vd[i].y, vd[i].z, vd[i].w}, g4[4] = {vg[i].x, vg[i].y, vg[i].z, vg[i].w},
+                    u4[4] = {vu[i].x, vu[i].y, vu[i].z, vu[i].w};
+        float rg[4], ru[4], rh[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float s = sigmoid_f32(g4[c]), silu = g4[c] * s, h = silu * u4[c], d = w * d4[c];
+          dot = fmaf(h, d4[c], dot);
+          ru[c] = d * silu;
+          rg[c] = d * u4[c] * fmaf(silu, 1.0f - s, s);
+          rh[c] = w * h;
+        }
+        odg = make_uint2(pack2<T>(rg[0], rg[1]), pack2<T>(rg[2], rg[3]));
+        odu = make_uint2(pack2<T>(ru[0], ru[1]), pack2<T>(ru[2], ru[3]));
+        ohs = make_uint2(pack2<T>(rh[0], rh[1]), pack2<T>(rh[2], rh[3]));
+      }
+      const int64_t at = row * vecs + v;
+      dg[at] = odg;
+      du[at] = odu;
+      if (hs != nullptr) hs[at] = ohs;
+    }
   }
   if (dweights == nullptr || pair < 0) return;
   __shared__ float part[8];
@@ -369,7 +385,7 @@ int gather_rows(const ExpertPlan& p, const int* plan, const void* src, void* dst
   return FSW_OK;
 }
 
-template <typename T>
+template <typename T, typename S>
 static cudaError_t launch_combine(const ExpertPlan& p, const int* plan, const void* src, const void* weights, int wtype,
                                   void* y, int vecs, cudaStream_t st) {
   const uint4* s = static_cast<const uint4*>(src);
@@ -377,29 +393,29 @@ static cudaError_t launch_combine(const ExpertPlan& p, const int* plan, const vo
   // a row per block; a row of few tokens is cut into pieces so that the GPU has some to do
   dim3 grid(p.T, p.T >= 512 ? 1 : (vecs + 127) / 128);
   if (weights == nullptr)
-    return launch_dependent(combine_kernel<T, float, false>, grid, 128, 0, st, true, 1, p, plan, s, weights, o, vecs);
+    return launch_dependent(combine_kernel<T, float, false, S>, grid, 128, 0, st, true, 1, p, plan, s, weights, o, vecs);
   if (wtype == FSW_FP32)
-    return launch_dependent(combine_kernel<T, float, true>, grid, 128, 0, st, true, 1, p, plan, s, weights, o, vecs);
-  return launch_dependent(combine_kernel<T, T, true>, grid, 128, 0, st, true, 1, p, plan, s, weights, o, vecs);
+    return launch_dependent(combine_kernel<T, float, true, S>, grid, 128, 0, st, true, 1, p, plan, s, weights, o, vecs);
+  return launch_dependent(combine_kernel<T, T, true, S>, grid, 128, 0, st, true, 1, p, plan, s, weights, o, vecs);
 }
 
-int combine_rows(const ExpertPlan& p, const int* plan, const void* src, const void* weights, int wtype, void* y,
+int combine_rows(const ExpertPlan& p, const int* plan, const void* src, bool src_f32, const void* weights, int wtype, void* y,
                  int64_t cols, int dtype, cudaStream_t st) {
-  if (dtype == FSW_BF16)
-    FSW_CUDA(launch_combine<__nv_bfloat16>(p, plan, src, weights, wtype, y, (int)(cols / 8), st));
-  else
-    FSW_CUDA(launch_combine<__half>(p, plan, src, weights, wtype, y, (int)(cols / 8), st));
+  auto* run = dtype == FSW_BF16
+                  ? (src_f32 ? launch_combine<__nv_bfloat16, float> : launch_combine<__nv_bfloat16, __nv_bfloat16>)
+                  : (src_f32 ? launch_combine<__half, float> : launch_combine<__half, __half>);
+  FSW_CUDA(run(p, plan, src, weights, wtype, y, (int)(cols / 8), st));
   return FSW_OK;
 }
 
 template <typename T, typename W>
-static int launch_gate(const ExpertPlan& p, const int* plan, void* dh, const void* g, const void* u, const void* weights,
-                       void* du, void* hs, void* dweights, int64_t cols, cudaStream_t st) {
-  const int vecs = (int)(cols / 8);
-  const int threads = vecs >= 256 ? 256 : vecs > 64 ? 128 : 64;
+static int launch_gate(const ExpertPlan& p, const int* plan, const void* dh, const void* g, const void* u, const void* weights,
+                       void* dg, void* du, void* hs, void* dweights, int64_t cols, cudaStream_t st) {
+  const int vecs = (int)(cols / 4);
+  const int threads = vecs >= 512 ? 256 : vecs > 128 ? 128 : 64;
   FSW_CUDA(launch_dependent(expert_gate_kernel<T, W>, dim3(p.rows), threads, 0, st, true, 1, p, plan,
-                            static_cast<uint4*>(dh), static_cast<const uint4*>(g), static_cast<const uint4*>(u), weights,
-                            static_cast<uint4*>(du), static_cast<uint4*>(hs), dweights, vecs));
+                            static_cast<const float4*>(dh), static_cast<const float4*>(g), static_cast<const float4*>(u),
+                            weights, static_cast<uint2*>(dg), static_cast<uint2*>(du), static_cast<uint2*>(hs), dweights, vecs));
   if (dweights != nullptr)
     FSW_CUDA(launch_dependent(dropped_weights_kernel<W>, dim3((p.pairs + 255) / 256), 256, 0, st, true, 1, p, plan,
                               static_cast<W*>(dweights)));
@@ -528,11 +544,7 @@ struct Experts {
     if ((rc = make_map(&p.b0, wg, dtype, f, d, 64, "w_gate", 64, 0, plan.E)) != FSW_OK) return rc;
     if ((rc = make_map(&p.b1, wu, dtype, f, d, 64, "w_up", 64, 0, plan.E)) != FSW_OK) return rc;
     if ((rc = make_map(&p.so, h, dtype, f, plan.rows, 32, "h", 32)) != FSW_OK) return rc;
-    p.sg = p.su = p.so;
-    if (g != nullptr) {
-      if ((rc = make_map(&p.sg, g, dtype, f, plan.rows, 32, "g", 32)) != FSW_OK) return rc;
-      if ((rc = make_map(&p.su, u, dtype, f, plan.rows, 32, "u", 32)) != FSW_OK) return rc;
-    }
+    p.sg = p.su = p.so;  // g and u are written by plain stores
     p.store_gu = g != nullptr;
     p.c0_ptr = g;
     p.c1_ptr = u;
@@ -603,24 +615,25 @@ static int check_16bit(int64_t T, int k, int E, int64_t d, int64_t f, int64_t d_
 struct ExpertBuffers {
   int64_t xs, g, u, saved;        // saved: plan at 0
   int64_t h, ys, scratch;         // forward scratch (training: h, ys; inference: plus plan and xs)
-  int64_t dys, dh, du, hs, dxs, back;  // backward scratch
+  int64_t dys, dh, dg, du, hs, dxs, back;  // backward scratch; dxs takes dh's place
 };
 static ExpertBuffers expert_buffers(const ExpertPlan& p, int64_t d, int64_t f, int64_t d_out) {
   ExpertBuffers b;
   const int64_t R = p.rows;
   b.xs = align256(p.ints * 4);
   b.g = b.xs + align256(R * d * 2);
-  b.u = b.g + align256(R * f * 2);
-  b.saved = b.u + align256(R * f * 2);
+  b.u = b.g + align256(R * f * 4);
+  b.saved = b.u + align256(R * f * 4);
   b.h = 0;
   b.ys = align256(R * f * 2);
-  b.scratch = b.ys + align256(R * d_out * 2);
+  b.scratch = b.ys + align256(R * d_out * 4);
   b.dys = 0;
   b.dh = align256(R * d_out * 2);
-  b.du = b.dh + align256(R * f * 2);
+  b.dxs = b.dh;
+  b.dg = b.dh + align256(R * (f > d ? f : d) * 4);
+  b.du = b.dg + align256(R * f * 2);
   b.hs = b.du + align256(R * f * 2);
-  b.dxs = b.hs + align256(R * f * 2);
-  b.back = b.dxs + align256(R * d * 2);
+  b.back = b.hs + align256(R * f * 2);
   return b;
 }
 
@@ -679,7 +692,7 @@ int fsw_experts_forward(const void* x, const void* weights, const void* indices,
   if ((rc = x_.swiglu(keep + b.xs, w_gate, w_up, tmp + b.h, train ? keep + b.g : nullptr, train ? keep + b.u : nullptr)) != FSW_OK)
     return rc;
   if ((rc = x_.product<MODE_GNN>(tmp + b.h, w_down, tmp + b.ys, f, d_out, false)) != FSW_OK) return rc;
-  return combine_rows(x_.plan, plan, tmp + b.ys, weights, weights_dtype, y, d_out, dtype, x_.st);
+  return combine_rows(x_.plan, plan, tmp + b.ys, true, weights, weights_dtype, y, d_out, dtype, x_.st);
 }
 
 int fsw_experts_backward(const void* dy, const void* weights, const void* w_gate, const void* w_up, const void* w_down,
@@ -725,12 +738,12 @@ int fsw_experts_backward(const void* dy, const void* weights, const void* w_gate
   const bool w32 = weights_dtype == FSW_FP32;
   auto* gate = dtype == FSW_BF16 ? (w32 ? launch_gate<__nv_bfloat16, float> : launch_gate<__nv_bfloat16, __nv_bfloat16>)
                                  : (w32 ? launch_gate<__half, float> : launch_gate<__half, __half>);
-  if ((rc = gate(x_.plan, plan, tmp + b.dh, keep + b.g, keep + b.u, weights, tmp + b.du, hs, dweights, f, st)) != FSW_OK) return rc;
-  const char *dg = tmp + b.dh, *du = tmp + b.du;  // dg took dh's place
+  if ((rc = gate(x_.plan, plan, tmp + b.dh, keep + b.g, keep + b.u, weights, tmp + b.dg, tmp + b.du, hs, dweights, f, st)) != FSW_OK) return rc;
+  const char *dg = tmp + b.dg, *du = tmp + b.du;
   if (dw_down && (rc = x_.grad_weight<MODE_GTN>(hs, tmp + b.dys, nullptr, dw_down, nullptr, f, d_out)) != FSW_OK) return rc;
   if (dx) {
     if ((rc = x_.grad_rows(dg, du, w_gate, w_up, tmp + b.dxs)) != FSW_OK) return rc;
-    if ((rc = combine_rows(x_.plan, plan, tmp + b.dxs, nullptr, FSW_FP32, dx, d, dtype, st)) != FSW_OK) return rc;
+    if ((rc = combine_rows(x_.plan, plan, tmp + b.dxs, true, nullptr, FSW_FP32, dx, d, dtype, st)) != FSW_OK) return rc;
   }
   if (dw_gate && (rc = x_.grad_weight<MODE_GDW>(keep + b.xs, dg, du, dw_gate, dw_up, d, f)) != FSW_OK) return rc;
   return FSW_OK;

@@ -63,8 +63,8 @@ int gather_rows(const ExpertPlan& p, const int* plan, const void* src, void* dst
                 bool zero_padding, bool dependent, cudaStream_t st);
 
 // y[t] = sum over j of weight[t, j] * src[row of (t, j)], in fp32, rounded once.
-// weights: nullptr for 1, else of type wtype (FSW_FP32 or dtype).
-int combine_rows(const ExpertPlan& p, const int* plan, const void* src, const void* weights, int wtype, void* y,
+// src: of type dtype or, with src_f32, fp32.  weights: nullptr for 1, else of type wtype (FSW_FP32 or dtype).
+int combine_rows(const ExpertPlan& p, const int* plan, const void* src, bool src_f32, const void* weights, int wtype, void* y,
                  int64_t cols, int dtype, cudaStream_t st);
 
 // The forward for a handful of tokens without the sort and the matrix kernels (fsw_few.cu);

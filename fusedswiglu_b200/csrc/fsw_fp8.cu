@@ -1029,7 +1029,7 @@ int fsw_fp8_experts_forward(const void* x, const void* weights, const void* indi
   if ((rc = run_fp8(r, hq, hs, 1, R, w_down, static_cast<const float*>(s_down), nullptr, nullptr, s + b.ys, nullptr, nullptr, f,
                     d_out, dtype, dev, st)) != FSW_OK)
     return rc;
-  return combine_rows(plan, plan_dev, s + b.ys, weights, weights_dtype, y, d_out, dtype, st);
+  return combine_rows(plan, plan_dev, s + b.ys, false, weights, weights_dtype, y, d_out, dtype, st);
 }
 
 }  // extern "C"

@@ -57,10 +57,10 @@ def run(x, w, idx, wg, wu, wd, dy=None):
     return out
 
 
-# Roundings between an input and each output: y passes g, u, h, its row and the sum
-# (5), dx dh, dg, du, its row and the sum on top of g and u (7), the weights' gradients at
-# most as many.  Each moves a value by HALF of it at most and, evenly spread over a step, by less
-# than half of that in the norm; they are independent: sqrt(7) * 0.5 HALF < 1.5 HALF.
+# 16-bit roundings between an input and each output: y passes h and its own, dx passes dg, du and
+# its own, a weight's gradient one operand and its own; 7 are allowed for.  Each moves a value by
+# HALF of it at most and, evenly spread over a step, by less than half of that in the norm; they
+# are independent: sqrt(7) * 0.5 HALF < 1.5 HALF.
 NAMES = ("y", "dx", "dweights", "dw_gate", "dw_up", "dw_down")
 
 
