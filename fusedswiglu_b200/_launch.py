@@ -331,8 +331,9 @@ def route(logits: torch.Tensor, bias: Optional[torch.Tensor], top_k: int, score:
     T, E = logits.shape
     if bias is not None:
         bias = bias.detach().to(torch.float32).contiguous()
-    weights = torch.empty((T, max(top_k, 0)), device=logits.device, dtype=torch.float32)
-    indices = torch.empty((T, max(top_k, 0)), device=logits.device, dtype=torch.int32)
+    k = min(max(top_k, 0), E)  # the call below refuses any other
+    weights = torch.empty((T, k), device=logits.device, dtype=torch.float32)
+    indices = torch.empty((T, k), device=logits.device, dtype=torch.int32)
     _call("fsw_route", logits,
           logits.data_ptr(), logits.stride(0) if T > 1 else E, bias.data_ptr() if bias is not None else None,
           weights.data_ptr(), indices.data_ptr(), T, E, top_k, code, _SCORE_CODE[score], int(renormalize), scale,

@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-enum { FSW_BF16 = 0, FSW_FP16 = 1, FSW_FP32 = 2 /* routing only */ };
+enum { FSW_BF16 = 0, FSW_FP16 = 1, FSW_FP32 = 2 /* routing; the weights of routed experts */ };
 enum { FSW_ACC_F32 = 0, FSW_ACC_F16 = 1 };
 enum {
   FSW_OK = 0,
