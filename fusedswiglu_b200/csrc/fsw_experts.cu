@@ -112,19 +112,18 @@ __device__ __forceinline__ void place_experts(const ExpertPlan& p, int* plan, in
 
 // Pairs of warp `warp` of block `block`: a contiguous range, a multiple of 32 long.
 __device__ __forceinline__ void warp_range(const ExpertPlan& p, int block, int warp, int& begin, int& end) {
-  const int per = kPlanChunk / kPlanWarps;
-  begin = block * kPlanChunk + warp * per;
-  end = begin + per < p.pairs ? begin + per : p.pairs;
+  begin = (block * p.warps + warp) * kPlanWarpPairs;
+  end = begin + kPlanWarpPairs < p.pairs ? begin + kPlanWarpPairs : p.pairs;
 }
 
 // Histogram per warp in shared memory; with `whole` the one block also places and ranks.
 template <bool whole>
-__global__ void __launch_bounds__(kPlanWarps * 32) plan_count_kernel(const ExpertPlan p, const int* indices, int* plan) {
-  extern __shared__ int hist[];  // [kPlanWarps][E]
-  __shared__ int warp_sums[kPlanWarps];
+__global__ void __launch_bounds__(1024) plan_count_kernel(const ExpertPlan p, const int* indices, int* plan) {
+  extern __shared__ int hist[];  // [warps][E]
+  __shared__ int warp_sums[32];
   ptx::allow_successor();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < kPlanWarps * p.E; i += blockDim.x) hist[i] = 0;
+  for (int i = threadIdx.x; i < p.warps * p.E; i += blockDim.x) hist[i] = 0;
   __syncthreads();
   int begin, end;
   warp_range(p, blockIdx.x, warp, begin, end);
@@ -132,7 +131,7 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_count_kernel(const Exper
   __syncthreads();
   auto total = [&](int e) {
     int c = 0;
-    for (int w = 0; w < kPlanWarps; ++w) c += hist[w * p.E + e];
+    for (int w = 0; w < p.warps; ++w) c += hist[w * p.E + e];
     return c;
   };
   if (!whole) {
@@ -143,7 +142,7 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_count_kernel(const Exper
   __syncthreads();
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
     int next = plan[p.offsets + e];
-    for (int w = 0; w < kPlanWarps; ++w) {
+    for (int w = 0; w < p.warps; ++w) {
       const int c = hist[w * p.E + e];
       hist[w * p.E + e] = next;
       next += c;
@@ -160,22 +159,28 @@ __global__ void __launch_bounds__(1024) plan_place_kernel(const ExpertPlan p, in
   ptx::wait_predecessor();
   place_experts(p, plan, warp_sums, [&](int e) {
     int c = 0;
-    for (int b = 0; b < p.blocks; ++b) {
-      int* h = plan + p.block_hist + (int64_t)b * p.E + e;
-      const int v = *h;
-      *h = c;
-      c += v;
+    int* h = plan + p.block_hist + e;
+    for (int b = 0; b < p.blocks; b += 8) {  // eight loads in flight
+      int v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = b + i < p.blocks ? h[(int64_t)(b + i) * p.E] : 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (b + i < p.blocks) {
+          h[(int64_t)(b + i) * p.E] = c;
+          c += v[i];
+        }
     }
     return c;
   });
 }
 
-__global__ void __launch_bounds__(kPlanWarps * 32) plan_rank_kernel(const ExpertPlan p, const int* indices, int* plan) {
+__global__ void __launch_bounds__(1024) plan_rank_kernel(const ExpertPlan p, const int* indices, int* plan) {
   extern __shared__ int hist[];
   ptx::allow_successor();
   ptx::wait_predecessor();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < kPlanWarps * p.E; i += blockDim.x) hist[i] = 0;
+  for (int i = threadIdx.x; i < p.warps * p.E; i += blockDim.x) hist[i] = 0;
   __syncthreads();
   int begin, end;
   warp_range(p, blockIdx.x, warp, begin, end);
@@ -183,7 +188,7 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rank_kernel(const Expert
   __syncthreads();
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
     int next = plan[p.offsets + e] + plan[p.block_hist + (int64_t)blockIdx.x * p.E + e];
-    for (int w = 0; w < kPlanWarps; ++w) {
+    for (int w = 0; w < p.warps; ++w) {
       const int c = hist[w * p.E + e];
       hist[w * p.E + e] = next;
       next += c;
@@ -366,8 +371,8 @@ __global__ void __launch_bounds__(256) dropped_weights_kernel(const ExpertPlan p
 }  // namespace
 
 int build_plan(const ExpertPlan& p, const int* indices, int* plan, cudaStream_t st) {
-  const size_t smem = sizeof(int) * kPlanWarps * p.E;  // at most 32 KB
-  const int threads = kPlanWarps * 32;
+  const size_t smem = sizeof(int) * p.warps * p.E;  // at most 45 KB
+  const int threads = p.warps * 32;
   if (p.blocks <= 1) {
     FSW_CUDA(launch_dependent(plan_count_kernel<true>, dim3(1), threads, smem, st, false, 1, p, indices, plan));
     return FSW_OK;

@@ -17,12 +17,12 @@
 
 namespace fsw {
 
-constexpr int kPlanChunk = 4096;   // pairs sorted by one block
-constexpr int kPlanWarps = 8;      // warps of a sorting block
+constexpr int kPlanWarpPairs = 128;  // pairs one warp of a sorting block takes, 32 at a time
 
 struct ExpertPlan {
   int T, k, E, tile_rows;
   int pairs, tiles, rows, blocks;
+  int warps;  // of a sorting block: 32, or 8 where 32 histograms of E counters would not fit 48 KB
   // offsets into the plan, in ints
   int64_t counts, offsets, tile_expert, pair_row, row_pair, block_hist, ints;
 };
@@ -32,7 +32,7 @@ inline bool make_plan(ExpertPlan* p, int64_t T, int k, int E, int tile_rows) {
   const int64_t pairs = T * k;
   const int64_t used = pairs < E ? pairs : E;
   const int64_t tiles = (pairs + used * (tile_rows - 1)) / tile_rows;
-  if (pairs >= (1ll << 31) || tiles * tile_rows >= (1ll << 31) - 1024) return false;
+  if (pairs >= (1ll << 31) - 8192 || tiles * tile_rows >= (1ll << 31) - 1024) return false;
   p->T = (int)T;
   p->k = k;
   p->E = E;
@@ -40,7 +40,8 @@ inline bool make_plan(ExpertPlan* p, int64_t T, int k, int E, int tile_rows) {
   p->pairs = (int)pairs;
   p->tiles = (int)tiles;
   p->rows = (int)(tiles * tile_rows);
-  p->blocks = (int)((pairs + kPlanChunk - 1) / kPlanChunk);
+  p->warps = E <= 352 ? 32 : 8;
+  p->blocks = (int)((pairs + p->warps * kPlanWarpPairs - 1) / (p->warps * kPlanWarpPairs));
   p->counts = 8;
   p->offsets = p->counts + E;
   p->tile_expert = p->offsets + E + 1;

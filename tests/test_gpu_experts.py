@@ -73,7 +73,7 @@ def compare(got, want, dtype):
 SHAPES = [  # T, E, k, d, f, o
     (1, 8, 2, 64, 64, 64), (3, 64, 6, 136, 72, 200), (33, 4, 4, 256, 128, 256), (130, 5, 3, 72, 264, 8),
     (500, 60, 4, 264, 136, 264), (1500, 4, 2, 512, 384, 512), (2000, 2, 1, 256, 1032, 520), (64, 1, 1, 128, 128, 128),
-    (700, 3, 2, 8, 8, 8),
+    (700, 3, 2, 8, 8, 8), (600, 400, 3, 16, 24, 16), (2100, 352, 2, 16, 16, 16),
 ]
 
 
