@@ -15,6 +15,12 @@
 // pair); in 512 cycles of MMAs per block and pair the epilogue reads 128 x 256 sums per SM
 // from tensor memory (256 cycles) and issues 128 packed FMAs per scheduler.
 //
+// Measured on one B200: 8192 x 4096 -> 14336 432 us (2.2 PFLOP/s) alone, where the same kernel without
+// the scaling takes 323 us; 77 x 14336 -> 4104 23 us; one token 4096 -> 14336 19 us with its
+// quantisation.  Bound by the epilogue: a warp needs about 575 cycles from a block's sums to their
+// release and 235 to the next, next to 512 of MMAs.  256-column MMAs with two regions: four
+// regions of 128 would hide more, but read the rows twice as often from shared memory (580 us).
+//
 // Few rows: the A box holds only the rows there are, and with fewer tiles than SMs the K
 // blocks of a tile are divided over the CTAs of a cluster, which add their sums through
 // distributed shared memory in a fixed order.

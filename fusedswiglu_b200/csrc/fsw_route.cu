@@ -7,8 +7,9 @@
 //
 // One warp per token; expert e sits in lane e % 32, so a row is read once, coalesced, and
 // lives in registers.  Selection is k rounds of redux.sync over order-preserving 32-bit
-// keys.  The bytes (T*E logits in, T*k*8 out) would take 2.6 us for 16384 x 256 fp32
-// logits; the rounds of dependent warp reductions bound the kernel, see route_kernel.
+// keys.  The bytes (T*E logits in, T*k*8 out) would take 2.7 us for 16384 x 256 fp32
+// logits; instructions bound the kernel.  Measured on one B200: 13 us for the top 8 of these,
+// 27 with a bias, 37 with a bias and 4 of 8 groups; 8191 x 128 bf16 7.1 us, its gradient 5.9.
 //
 // The selection is that of exact arithmetic.  Without a bias s grows with z, so z itself is
 // compared and nothing is rounded.  With a bias, or for group scores, c is computed in
