@@ -134,6 +134,8 @@ class RouterLogits(Function):
         dw = None
         if ctx.needs_input_grad[1]:
             T = x2d.shape[0]
+            if T == 0:
+                return dx, torch.zeros_like(w)
             if T % 8:  # the GEMM wants the transposed operand's rows in multiples of 8: rows of zeros add nothing
                 pad = 8 - T % 8
                 x2d = torch.cat([x2d, x2d.new_zeros(pad, x2d.shape[1])])

@@ -41,22 +41,26 @@ class FusedRouter(Function):
     def forward(ctx, logits, bias, top_k, score, renormalize, scale, num_groups, topk_groups):
         z, weights, indices = _forward(logits, bias, top_k, score, renormalize, scale, num_groups, topk_groups)
         ctx.save_for_backward(z, indices)
+        ctx.set_materialize_grads(False)  # no zeros for the indices' gradient
         ctx.args = (score, bool(renormalize), float(scale))
         ctx.in_shape = logits.shape
-        shape = logits.shape[:-1] + (int(top_k),)
-        out = indices.view(shape)
-        ctx.mark_non_differentiable(out)
-        return weights.view(shape), out
+        if logits.ndim != 2:
+            shape = logits.shape[:-1] + (int(top_k),)
+            weights, indices = weights.view(shape), indices.view(shape)
+        ctx.mark_non_differentiable(indices)
+        return weights, indices
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_weights, _grad_indices):
         dz = None
-        if ctx.needs_input_grad[0]:
+        if ctx.needs_input_grad[0] and grad_weights is not None:
             z, indices = ctx.saved_tensors
             score, renormalize, scale = ctx.args
             dw = grad_weights.reshape(indices.shape).contiguous()
-            dz = _launch.route_backward(z, indices, dw, score, renormalize, scale).view(ctx.in_shape)
+            dz = _launch.route_backward(z, indices, dw, score, renormalize, scale)
+            if len(ctx.in_shape) != 2:
+                dz = dz.view(ctx.in_shape)
         return dz, None, None, None, None, None, None, None
 
 

@@ -163,6 +163,18 @@ def test_layers_in_a_row_with_a_padded_batch():
         assert (a[T:] == 0).all()
 
 
+def test_a_block_without_tokens():
+    from fusedswiglu_b200 import Fp8SwiGLUMoE, SwiGLUMoE
+
+    m = SwiGLUMoE(64, 64, 8, 2, device="cuda")
+    x = torch.zeros(3, 0, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = m(x)
+    y.sum().backward()
+    assert y.shape == x.shape == x.grad.shape
+    assert all((p.grad == 0).all() and p.grad.shape == p.shape for p in m.parameters())
+    assert Fp8SwiGLUMoE(m)(x.detach()).shape == x.shape
+
+
 def test_shared_and_broadcast_inputs_get_summed_gradients():
     from fusedswiglu_b200 import FusedSwiGLUExperts
 
