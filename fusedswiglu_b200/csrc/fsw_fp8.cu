@@ -270,153 +270,153 @@ __global__ void __launch_bounds__(Fp8Cfg<CG>::THREADS, 1) fp8_gemm_kernel(const 
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_FIRST));
-   if (warp == 0) {
-    // ======================= TMA producer (one thread) =======================
-    if (lane == 0 && !p.stall_producer) {
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      const uint64_t pol = ptx::make_l2_policy(2);
-      const uint32_t bytes = CG * (static_cast<uint32_t>(p.a_rows) * kBlock + C::B_BYTES);
-      Fp8Work w;
-      auto row_of = [&]() { return w.m_tile * 128 * CG + (CG == 2 ? static_cast<int>(rank) * 128 : 0); };
-      auto bar_of = [&](int st) { return CG == 2 ? ptx::mapa(full_bar(st), 0) : full_bar(st); };
-      auto load_rows = [&](int kb, int st) {
-        const uint32_t dst = smem_base + st * C::STAGE_BYTES;
-        if constexpr (CG == 2)
-          ptx::tma_load_2d_pair(dst, &p.a, bar_of(st), kb * kBlock, row_of(), pol);
-        else
-          ptx::tma_load_2d(dst, &p.a, full_bar(st), kb * kBlock, row_of(), pol);
-      };
-      auto load_weight = [&](int kb, int st) {
-        const uint32_t dst = smem_base + st * C::STAGE_BYTES + C::A_BYTES;
-        const int k0 = kb * kBlock, n0 = w.n_tile * (DUAL ? 128 : 256);
-        if (CG == 1 || rank == 0) ptx::mbar_arrive_expect_tx(full_bar(st), bytes);
-        if constexpr (CG == 2) {
-          // each CTA stages one half of the tile's weight rows
-          ptx::tma_load_3d_pair(dst, (DUAL && rank) ? &p.b1 : &p.b0, bar_of(st), k0,
-                                DUAL ? n0 : n0 + static_cast<int>(rank) * 128, w.expert, pol);
-        } else {
-          ptx::tma_load_3d(dst, &p.b0, full_bar(st), k0, n0, w.expert, pol);
-          ptx::tma_load_3d(dst + 128 * kBlock, DUAL ? &p.b1 : &p.b0, full_bar(st), k0, DUAL ? n0 : n0 + 128, w.expert, pol);
-        }
-      };
-      int ahead = 0;  // blocks of the first tile whose weight tiles are on their way
-      if (early) {
-        if (get_work(0, w)) {
-          ahead = kb1 - kb0 < STAGES ? kb1 - kb0 : STAGES;
-          for (int i = 0; i < ahead; ++i) load_weight(kb0 + i, i);
-        }
-        ptx::wait_predecessor();
-      }
-      for (int idx = 0; ok && get_work(idx, w); ++idx) {
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (ahead > 0) {
-            --ahead;  // the pipeline is empty: stage s is kb - kb0
+    if (warp == 0) {
+      // ======================= TMA producer (one thread) =======================
+      if (lane == 0 && !p.stall_producer) {
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        const uint64_t pol = ptx::make_l2_policy(2);
+        const uint32_t bytes = CG * (static_cast<uint32_t>(p.a_rows) * kBlock + C::B_BYTES);
+        Fp8Work w;
+        auto row_of = [&]() { return w.m_tile * 128 * CG + (CG == 2 ? static_cast<int>(rank) * 128 : 0); };
+        auto bar_of = [&](int st) { return CG == 2 ? ptx::mapa(full_bar(st), 0) : full_bar(st); };
+        auto load_rows = [&](int kb, int st) {
+          const uint32_t dst = smem_base + st * C::STAGE_BYTES;
+          if constexpr (CG == 2)
+            ptx::tma_load_2d_pair(dst, &p.a, bar_of(st), kb * kBlock, row_of(), pol);
+          else
+            ptx::tma_load_2d(dst, &p.a, full_bar(st), kb * kBlock, row_of(), pol);
+        };
+        auto load_weight = [&](int kb, int st) {
+          const uint32_t dst = smem_base + st * C::STAGE_BYTES + C::A_BYTES;
+          const int k0 = kb * kBlock, n0 = w.n_tile * (DUAL ? 128 : 256);
+          if (CG == 1 || rank == 0) ptx::mbar_arrive_expect_tx(full_bar(st), bytes);
+          if constexpr (CG == 2) {
+            // each CTA stages one half of the tile's weight rows
+            ptx::tma_load_3d_pair(dst, (DUAL && rank) ? &p.b1 : &p.b0, bar_of(st), k0,
+                                  DUAL ? n0 : n0 + static_cast<int>(rank) * 128, w.expert, pol);
           } else {
-            ok = bounded_wait_thread(empty_bar(s), ph ^ 1u, ctl, WAIT_PRODUCER_EMPTY);
-            if (!ok) break;
-            load_weight(kb, s);
+            ptx::tma_load_3d(dst, &p.b0, full_bar(st), k0, n0, w.expert, pol);
+            ptx::tma_load_3d(dst + 128 * kBlock, DUAL ? &p.b1 : &p.b0, full_bar(st), k0, DUAL ? n0 : n0 + 128, w.expert, pol);
           }
-          load_rows(kb, s);
-          if (++s == STAGES) {
-            s = 0;
-            ph ^= 1u;
+        };
+        int ahead = 0;  // blocks of the first tile whose weight tiles are on their way
+        if (early) {
+          if (get_work(0, w)) {
+            ahead = kb1 - kb0 < STAGES ? kb1 - kb0 : STAGES;
+            for (int i = 0; i < ahead; ++i) load_weight(kb0 + i, i);
+          }
+          ptx::wait_predecessor();
+        }
+        for (int idx = 0; ok && get_work(idx, w); ++idx) {
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (ahead > 0) {
+              --ahead;  // the pipeline is empty: stage s is kb - kb0
+            } else {
+              ok = bounded_wait_thread(empty_bar(s), ph ^ 1u, ctl, WAIT_PRODUCER_EMPTY);
+              if (!ok) break;
+              load_weight(kb, s);
+            }
+            load_rows(kb, s);
+            if (++s == STAGES) {
+              s = 0;
+              ph ^= 1u;
+            }
           }
         }
       }
-    }
-   } else if (warp == 1) {
-    // ================ MMA issuer (one thread of the pair leader) ================
-    if ((CG == 1 || rank == 0) && lane == 0) {
-      int s = 0, a = 0;
-      uint32_t ph = 0, aph = 0;
+    } else if (warp == 1) {
+      // ================ MMA issuer (one thread of the pair leader) ================
+      if ((CG == 1 || rank == 0) && lane == 0) {
+        int s = 0, a = 0;
+        uint32_t ph = 0, aph = 0;
+        bool ok = true;
+        auto commit = [&](uint32_t bar) {
+          if (CG == 2)
+            ptx::mma_commit_pair(bar, 3);
+          else
+            ptx::mma_commit(bar);
+        };
+        Fp8Work w;
+        for (int idx = 0; ok && get_work(idx, w); ++idx) {
+          for (int kb = kb0; kb < kb1; ++kb) {
+            ok = bounded_wait_thread(full_bar(s), ph, ctl, WAIT_MMA_FULL);
+            if (!ok) break;
+            ok = bounded_wait_thread(tempty_bar(a), aph ^ 1u, ctl, WAIT_MMA_TMEM_EMPTY);
+            if (!ok) break;
+            ptx::tc_fence_after_sync();
+            const uint32_t a_addr = smem_base + s * C::STAGE_BYTES, b_addr = a_addr + C::A_BYTES;
+#pragma unroll
+            for (int k = 0; k < kBlock / 32; ++k)
+              mma_f8_ss<CG>(tmem_base + a * 256, p.desc | (((a_addr + k * 32u) & 0x3FFFFu) >> 4),
+                            p.desc | (((b_addr + k * 32u) & 0x3FFFFu) >> 4), p.idesc, k != 0 ? 1u : 0u);
+            commit(tfull_bar(a));
+            commit(empty_bar(s));
+            a ^= 1;
+            if (a == 0) aph ^= 1u;
+            if (++s == STAGES) {
+              s = 0;
+              ph ^= 1u;
+            }
+          }
+        }
+      }
+    } else if (warp == 2) {
+      // ================ scales of each block's rows, for the epilogue ================
+      // Slot kb % 4 is written once the MMAs of block kb - 2 are complete: they began after the
+      // epilogue had finished with block kb - 4.  Global loads run kAhead blocks ahead: a load
+      // asked for one block before its use cost more time than the block's MMAs.
+      constexpr int kAhead = 4;
+      int n = 0;  // blocks of all tiles so far
       bool ok = true;
-      auto commit = [&](uint32_t bar) {
-        if (CG == 2)
-          ptx::mma_commit_pair(bar, 3);
-        else
-          ptx::mma_commit(bar);
-      };
       Fp8Work w;
       for (int idx = 0; ok && get_work(idx, w); ++idx) {
-        for (int kb = kb0; kb < kb1; ++kb) {
-          ok = bounded_wait_thread(full_bar(s), ph, ctl, WAIT_MMA_FULL);
-          if (!ok) break;
-          ok = bounded_wait_thread(tempty_bar(a), aph ^ 1u, ctl, WAIT_MMA_TMEM_EMPTY);
-          if (!ok) break;
-          ptx::tc_fence_after_sync();
-          const uint32_t a_addr = smem_base + s * C::STAGE_BYTES, b_addr = a_addr + C::A_BYTES;
+        const int row0 = w.m_tile * 128 * CG + (CG == 2 ? static_cast<int>(rank) * 128 : 0);
+        const float* x[4];
 #pragma unroll
-          for (int k = 0; k < kBlock / 32; ++k)
-            mma_f8_ss<CG>(tmem_base + a * 256, p.desc | (((a_addr + k * 32u) & 0x3FFFFu) >> 4),
-                          p.desc | (((b_addr + k * 32u) & 0x3FFFFu) >> 4), p.idesc, k != 0 ? 1u : 0u);
-          commit(tfull_bar(a));
-          commit(empty_bar(s));
-          a ^= 1;
-          if (a == 0) aph ^= 1u;
-          if (++s == STAGES) {
-            s = 0;
-            ph ^= 1u;
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int row = row0 + i * 32 + lane;
+          x[i] = p.xs + static_cast<int64_t>(row < p.M ? row : p.M - 1) * p.xs_row;
         }
-      }
-    }
-   } else if (warp == 2) {
-    // ================ scales of each block's rows, for the epilogue ================
-    // Slot kb % 4 is written once the MMAs of block kb - 2 are complete: they began after the
-    // epilogue had finished with block kb - 4.  Global loads run kAhead blocks ahead: a load
-    // asked for one block before its use cost more time than the block's MMAs.
-    constexpr int kAhead = 4;
-    int n = 0;  // blocks of all tiles so far
-    bool ok = true;
-    Fp8Work w;
-    for (int idx = 0; ok && get_work(idx, w); ++idx) {
-      const int row0 = w.m_tile * 128 * CG + (CG == 2 ? static_cast<int>(rank) * 128 : 0);
-      const float* x[4];
+        const int nb = DUAL ? w.n_tile : 2 * w.n_tile;
+        const int64_t wbase = (static_cast<int64_t>(w.expert) * p.ws_rows + nb) * p.num_kb;
+        const float* w0 = p.ws0 + wbase;
+        // the second block of a tile may lie behind the weight's last
+        const float* w1 = DUAL ? p.ws1 + wbase : (nb + 1 < p.ws_rows ? w0 + p.num_kb : w0);
+        float xv[kAhead][4], wv[kAhead][2];
+        auto fetch = [&](int kb, int i) {
+          kb = kb < kb1 ? kb : kb1 - 1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = row0 + i * 32 + lane;
-        x[i] = p.xs + static_cast<int64_t>(row < p.M ? row : p.M - 1) * p.xs_row;
-      }
-      const int nb = DUAL ? w.n_tile : 2 * w.n_tile;
-      const int64_t wbase = (static_cast<int64_t>(w.expert) * p.ws_rows + nb) * p.num_kb;
-      const float* w0 = p.ws0 + wbase;
-      // the second block of a tile may lie behind the weight's last
-      const float* w1 = DUAL ? p.ws1 + wbase : (nb + 1 < p.ws_rows ? w0 + p.num_kb : w0);
-      float xv[kAhead][4], wv[kAhead][2];
-      auto fetch = [&](int kb, int i) {
-        kb = kb < kb1 ? kb : kb1 - 1;
+          for (int r = 0; r < 4; ++r) xv[i][r] = x[r][kb * p.xs_block];
+          wv[i][0] = w0[kb];
+          wv[i][1] = w1[kb];
+        };
 #pragma unroll
-        for (int r = 0; r < 4; ++r) xv[i][r] = x[r][kb * p.xs_block];
-        wv[i][0] = w0[kb];
-        wv[i][1] = w1[kb];
-      };
+        for (int i = 0; i < kAhead; ++i) fetch(kb0 + i, i);
+        for (int kbase = kb0; kbase < kb1 && ok; kbase += kAhead) {
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) fetch(kb0 + i, i);
-      for (int kbase = kb0; kbase < kb1 && ok; kbase += kAhead) {
+          for (int i = 0; i < kAhead; ++i) {
+            if (kbase + i < kb1 && ok) {
+              // block n - 2 used the same region: its phase is the one before
+              if (n >= 2) ok = bounded_wait_warp(tfull_bar(n & 1), ((n >> 1) - 1) & 1, ctl, WAIT_EPI_TMEM_FULL);
+              if (ok) {
+                float* slot = scale_ring + (n & 3) * 256 + lane;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          if (kbase + i < kb1 && ok) {
-            // block n - 2 used the same region: its phase is the one before
-            if (n >= 2) ok = bounded_wait_warp(tfull_bar(n & 1), ((n >> 1) - 1) & 1, ctl, WAIT_EPI_TMEM_FULL);
-            if (ok) {
-              float* slot = scale_ring + (n & 3) * 256 + lane;
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                slot[r * 32] = xv[i][r] * wv[i][0];
-                slot[128 + r * 32] = xv[i][r] * wv[i][1];
+                for (int r = 0; r < 4; ++r) {
+                  slot[r * 32] = xv[i][r] * wv[i][0];
+                  slot[128 + r * 32] = xv[i][r] * wv[i][1];
+                }
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(tfull_bar(n & 1));
+                ++n;
+                fetch(kbase + i + kAhead, i);
               }
-              __syncwarp();
-              if (lane == 0) ptx::mbar_arrive(tfull_bar(n & 1));
-              ++n;
-              fetch(kbase + i + kAhead, i);
             }
           }
         }
       }
     }
-   }
   } else {
     // ======================= epilogue: scale, add, write =======================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_EPILOGUE));
@@ -700,6 +700,12 @@ int launch_fp8_one(const Fp8Params& p, int grid, bool dependent, cudaStream_t st
   if (!(prepared.load() >> (dev & 63) & 1)) {
     FSW_CUDA(cudaFuncSetAttribute(fp8_gemm_kernel<CG, DUAL, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   Fp8Cfg<CG>::SMEM_BYTES));
+    // The warpgroups trade registers within what the block is launched with; a build that
+    // launches with fewer would leave the epilogue waiting for its share.
+    cudaFuncAttributes attr;
+    FSW_CUDA(cudaFuncGetAttributes(&attr, fp8_gemm_kernel<CG, DUAL, T>));
+    if (attr.numRegs * Fp8Cfg<CG>::THREADS < Fp8Cfg<CG>::REGS_FIRST * 128 + Fp8Cfg<CG>::REGS_EPILOGUE * 32 * Fp8Cfg<CG>::EPI_WARPS)
+      return fail(FSW_EUNAVAILABLE, "the 8-bit kernel was built with %d registers a thread", attr.numRegs);
     prepared.fetch_or(1ull << (dev & 63));
   }
   FSW_CUDA(launch_dependent(fp8_gemm_kernel<CG, DUAL, T>, dim3(grid), Fp8Cfg<CG>::THREADS, Fp8Cfg<CG>::SMEM_BYTES, st,
